@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define SCREEN_ABI_VERSION 5
+#define SCREEN_ABI_VERSION 6
 
 #if defined(__GNUC__)
 #define SCREEN_API __attribute__((visibility("default")))
@@ -47,7 +47,7 @@ extern "C" {
 
 typedef void* screen_stream_t; /* a cudaStream_t; NULL = legacy default stream */
 
-enum screen_dtype { SCREEN_F32 = 0, SCREEN_BF16 = 1 };
+enum screen_dtype { SCREEN_F32 = 0, SCREEN_BF16 = 1, SCREEN_I8 = 2 /* cache pages only */ };
 
 enum screen_status {
   SCREEN_OK = 0,
@@ -254,6 +254,135 @@ SCREEN_API int screen_decode_append(const screen_kv_append_args* ap, const scree
 SCREEN_API int screen_decode_noalloc(const screen_decode_args* a, screen_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Speculative serving on the paged cache.  No counterpart in the reference,  */
+/* whose generate() recomputes the prefix for every token (model.py:131-133). */
+/*                                                                            */
+/* int8 pages.  A row holds m = round_half_even(127 x / max|x|) of the raw    */
+/* row x and scale = 1 / max(|m|, 127 eps / max|x|): scale * m is the unit    */
+/* form of the rounded raw row.  Scales are fp32 [num_pages, H, page_size].   */
+/* A row with an infinity or NaN is stored as m = 0, scale = NaN.             */
+/* In every call here positions outside the block table, and page ids outside */
+/* the cache, are skipped (nothing written, rows read as 0 or not seen).      */
+/* ------------------------------------------------------------------------ */
+typedef struct screen_paged_append_args {
+  int32_t dtype;                 /* of k, v: SCREEN_F32 / SCREEN_BF16          */
+  int32_t B, H, D, n_new;
+  float eps;
+  const void* k; int64_t k_sb, k_st;   /* raw (B,n_new,H,D)                   */
+  const void* v; int64_t v_sb, v_st;
+  const int32_t* positions;      /* (B,) position of row 0                    */
+  screen_kv_cache cache;         /* int8 pages                                */
+  float* k_scales; float* v_scales;
+} screen_paged_append_args;
+
+/* screen_kv_append for int8 pages. */
+SCREEN_API int screen_paged_append_i8(const screen_paged_append_args* a, screen_stream_t stream);
+
+typedef struct screen_paged_read_args {
+  int32_t dtype;                 /* of the rows written to k, v               */
+  int32_t cache_dtype;           /* SCREEN_F32 / SCREEN_BF16 / SCREEN_I8      */
+  int32_t B, H, D, n;
+  void* k; void* v;              /* (B,n,H,D) contiguous: the rows' values    */
+  const int32_t* positions;      /* (B,) position of row 0                    */
+  screen_kv_cache cache;
+  const float* k_scales; const float* v_scales;   /* int8 pages, else NULL    */
+} screen_paged_read_args;
+
+/* The values of n cached rows per sequence from positions[b] on. */
+SCREEN_API int screen_paged_read(const screen_paged_read_args* a, screen_stream_t stream);
+
+#define SCREEN_TREE_MAX_NODES 64
+
+typedef struct screen_tree_args {
+  int32_t dtype;                 /* of q, k, v, y                             */
+  int32_t cache_dtype;           /* = dtype, or SCREEN_I8                     */
+  int32_t B, H, D, n;            /* n <= SCREEN_TREE_MAX_NODES nodes          */
+  int32_t num_splits;            /* runs the key axis is cut into; >= 1       */
+  int32_t max_window;            /* keys a query is expected to see (<= 0:    */
+                                 /*   the table's length); sets the share of  */
+                                 /*   a split, not what is seen               */
+  float eps;
+  int32_t _pad0;
+  const void* q; int64_t q_sb, q_st;   /* raw (B,n,H,D)                       */
+  const void* k; int64_t k_sb, k_st;   /* raw rows of the nodes, or NULL:     */
+  const void* v; int64_t v_sb, v_st;   /*   they are in the cache already     */
+  const int32_t* lens;           /* (B,) cached tokens before the tree; < 0:  */
+                                 /*   an empty place (y = 0, nothing written) */
+  const int32_t* parents; int64_t parents_sb;  /* (B,n) or NULL: a chain      */
+  const float* r; const float* w;      /* (H,)                                */
+  screen_kv_cache cache;
+  float* k_scales; float* v_scales;    /* int8 pages, else NULL               */
+  void* y;                       /* (B,n,H,D) contiguous                      */
+  void* workspace; size_t workspace_bytes;
+} screen_tree_args;
+
+SCREEN_API size_t screen_tree_workspace_size(const screen_tree_args* a);
+
+/* Screening attention of a tree of n drafted tokens per sequence.  Node i has
+ * parents[b,i] in [-1, i) (-1: child of the newest cached token; any other
+ * value makes it absent, with all its descendants: y = 0, no row written).
+ * It owns cache position lens[b] + i, where its unit k / v rows are written
+ * first (k, v given), and stands at position lens[b] + depth: it sees the
+ * cached tokens of its window, its ancestors and itself.  A path of the tree
+ * thus gives what screen_decode_append gives token by token.  The ring of a
+ * sequence must hold ceil(w) - 1 + n rows. */
+SCREEN_API int screen_tree_decode(const screen_tree_args* a, screen_stream_t stream);
+
+/* One query per sequence at position lens[b] - 1 (the newest cached token)
+ * over int8 pages: screen_decode for the int8 cache.  a->n is 1, k / v /
+ * parents are NULL, q is (B,1,H,D). */
+SCREEN_API int screen_paged_decode_i8(const screen_tree_args* a, screen_stream_t stream);
+
+typedef struct screen_commit_args {
+  int32_t cache_dtype;
+  int32_t L, B, H, D, n;         /* L layers, n <= SCREEN_TREE_MAX_NODES      */
+  const int32_t* lens;           /* (B,) cached tokens before the tree        */
+  const int32_t* path; int64_t path_sb;   /* (B,n) accepted nodes in order    */
+  const int32_t* counts;         /* (B,) how many of them                     */
+  screen_kv_cache cache;         /* layer 0's pages                           */
+  float* k_scales; float* v_scales;
+  int64_t layer_stride;          /* rows of D elements from layer to layer    */
+} screen_commit_args;
+
+/* Row lens[b] + path[b,i] moved to lens[b] + i for i < counts[b], in all L
+ * layers; entries outside [0, n) leave their row as it is. */
+SCREEN_API int screen_paged_commit(const screen_commit_args* a, screen_stream_t stream);
+
+typedef struct screen_verify_args {
+  int32_t dtype;                 /* of the logits: SCREEN_F32 / SCREEN_BF16   */
+  int32_t B, n, V;               /* 0 <= n <= SCREEN_TREE_MAX_NODES           */
+  float temperature;             /* > 0; 0: greedy (the first maximum)        */
+  int32_t _pad0;
+  const float* temperatures;     /* (B,), or NULL: `temperature` for all      */
+  const void* logits; int64_t l_sb, l_st;        /* (B,n+1,V)                 */
+  const void* draft_logits; int64_t d_sb, d_st;  /* (B,n,V) or NULL           */
+  const int64_t* tokens; int64_t t_sb;           /* (B,n) drafted tokens      */
+  const int32_t* parents; int64_t p_sb;          /* (B,n) or NULL: a chain    */
+  const float* uniforms; int64_t u_sb;           /* (B,n+1) in [0, 1)         */
+  int64_t* out_tokens;           /* (B,n+1): the accepted tokens, one more    */
+                                 /*   drawn from the target, then -1          */
+  int32_t* path;                 /* (B,n): accepted nodes, then -1            */
+  int32_t* counts;               /* (B,): accepted nodes                      */
+  void* workspace; size_t workspace_bytes;
+} screen_verify_args;
+
+SCREEN_API size_t screen_verify_workspace_size(const screen_verify_args* a);
+
+/* Speculative sampling.  Logits row 0 follows the newest token, row 1 + i
+ * drafted token i; drafting row j is the distribution the children of row j
+ * were drawn from.  p, q: softmax(row / T).  Nodes are scanned in order; one
+ * whose parent is the current row is accepted iff
+ * u_i q(x) Z < p(x) - c q(x), and becomes the current row (c = 0, Z = 1);
+ * otherwise c += Z, Z = sum max(p - c q, 0).  Without drafting logits the
+ * tokens were picked: q(x) = 1, and a rejection takes x out of p.  Then one
+ * token is drawn from the residual, the first whose running sum passes
+ * u_n Z (from p if the residual is empty).  A target row without a finite
+ * maximum, or with a NaN, accepts nothing and gives token -1; from such a
+ * drafting row nothing is accepted.  A node outside the tree (see
+ * screen_tree_decode) or with a token outside [0, V) is never accepted. */
+SCREEN_API int screen_verify_drafts(const screen_verify_args* a, screen_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Few-row linear layer for the decode step of generate() (B <= 8 tokens):   */
 /* y[m, n] = act(sum_k xin[m, k] W[n, k]) (+ res[m, n]), bf16 in and out,    */
 /* fp32 accumulation.  xin = x, or RMSNorm(x) * norm_w when norm_w is given  */
@@ -377,7 +506,8 @@ SCREEN_API int screen_col_scale_bwd(int32_t dtype, int64_t rows, int32_t D, cons
 SCREEN_API const char* screen_strerror(int status);
 SCREEN_API int screen_version(void);                  /* SCREEN_ABI_VERSION             */
 /* sizeof of the argument structs, for binding checks: 0 fwd, 1 bwd,
- * 2 kv_cache, 3 kv_append, 4 decode, 5 rows_linear, 6 xent; -1 for an unknown id. */
+ * 2 kv_cache, 3 kv_append, 4 decode, 5 rows_linear, 6 xent, 7 rmsnorm, 16 paged_append,
+ * 17 paged_read, 18 tree, 19 commit, 20 verify; -1 for an unknown id. */
 SCREEN_API int64_t screen_sizeof_args(int which);
 /* Last CUDA error string seen by this thread inside the library. */
 SCREEN_API const char* screen_last_cuda_error(void);

@@ -19,6 +19,8 @@ from .kv_cache import PagedKVCache
 from .layers import MultiscreenBlock, MultiscreenDecoderLayer
 from .model import MultiscreenLM
 from .norm import TanhNorm
+from .paged import (paged_append, paged_commit, paged_decode, paged_read, paged_tree_decode,
+                    verify_drafts)
 from .sequence_parallel import (SequenceShard, current_shard, screening_attention_sharded,
                                 sequence_parallel, shard_timeline, shard_timeline_summary)
 from . import _lib
@@ -35,6 +37,12 @@ __all__ = [
     "screening_attention",
     "tanh_norm",
     "PagedKVCache",
+    "paged_append",
+    "paged_read",
+    "paged_decode",
+    "paged_tree_decode",
+    "paged_commit",
+    "verify_drafts",
     "sequence_parallel",
     "shard_timeline",
     "shard_timeline_summary",

@@ -114,6 +114,67 @@ class DecodeArgs(ctypes.Structure):
     ]
 
 
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("B", c_int32), ("H", c_int32), ("D", c_int32), ("n_new", c_int32),
+        ("eps", c_float),
+        ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64),
+        ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64),
+        ("positions", c_void_p), ("cache", KVCacheDesc),
+        ("k_scales", c_void_p), ("v_scales", c_void_p),
+    ]
+
+
+class PagedReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("cache_dtype", c_int32), ("B", c_int32), ("H", c_int32),
+        ("D", c_int32), ("n", c_int32), ("k", c_void_p), ("v", c_void_p),
+        ("positions", c_void_p), ("cache", KVCacheDesc),
+        ("k_scales", c_void_p), ("v_scales", c_void_p),
+    ]
+
+
+class TreeArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("cache_dtype", c_int32), ("B", c_int32), ("H", c_int32),
+        ("D", c_int32), ("n", c_int32), ("num_splits", c_int32), ("max_window", c_int32),
+        ("eps", c_float), ("_pad0", c_int32),
+        ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64),
+        ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64),
+        ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64),
+        ("lens", c_void_p), ("parents", c_void_p), ("parents_sb", c_int64),
+        ("r", c_void_p), ("w", c_void_p), ("cache", KVCacheDesc),
+        ("k_scales", c_void_p), ("v_scales", c_void_p), ("y", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class CommitArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache_dtype", c_int32), ("L", c_int32), ("B", c_int32), ("H", c_int32),
+        ("D", c_int32), ("n", c_int32),
+        ("lens", c_void_p), ("path", c_void_p), ("path_sb", c_int64), ("counts", c_void_p),
+        ("cache", KVCacheDesc), ("k_scales", c_void_p), ("v_scales", c_void_p),
+        ("layer_stride", c_int64),
+    ]
+
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("B", c_int32), ("n", c_int32), ("V", c_int32),
+        ("temperature", c_float), ("_pad0", c_int32), ("temperatures", c_void_p),
+        ("logits", c_void_p), ("l_sb", c_int64), ("l_st", c_int64),
+        ("draft_logits", c_void_p), ("d_sb", c_int64), ("d_st", c_int64),
+        ("tokens", c_void_p), ("t_sb", c_int64), ("parents", c_void_p), ("p_sb", c_int64),
+        ("uniforms", c_void_p), ("u_sb", c_int64),
+        ("out_tokens", c_void_p), ("path", c_void_p), ("counts", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+TREE_MAX_NODES = 64
+I8 = 2
+
 EXPORTED = (
     "screen_fwd", "screen_bwd", "screen_bwd_workspace_size", "screen_kv_append",
     "screen_decode", "screen_decode_workspace_size", "screen_tanhnorm_fwd",
@@ -123,8 +184,11 @@ EXPORTED = (
     "screen_cross_entropy_fwd", "screen_cross_entropy_bwd", "screen_rmsnorm_partials",
     "screen_rmsnorm_fwd", "screen_rmsnorm_bwd", "screen_head_params_fwd",
     "screen_head_params_bwd", "screen_col_scale_bwd", "screen_decode_append",
+    "screen_paged_append_i8", "screen_paged_read", "screen_tree_workspace_size",
+    "screen_tree_decode", "screen_paged_decode_i8", "screen_paged_commit",
+    "screen_verify_workspace_size", "screen_verify_drafts",
 )
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 _lib = None
 
@@ -169,6 +233,16 @@ def load() -> ctypes.CDLL:
     lib.screen_col_scale_bwd.argtypes = [c_int32, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p]
     lib.screen_decode_append.argtypes = [P(KVAppendArgs), P(DecodeArgs), c_void_p]
+    lib.screen_paged_append_i8.argtypes = [P(PagedAppendArgs), c_void_p]
+    lib.screen_paged_read.argtypes = [P(PagedReadArgs), c_void_p]
+    lib.screen_tree_workspace_size.argtypes = [P(TreeArgs)]
+    lib.screen_tree_workspace_size.restype = c_size_t
+    lib.screen_tree_decode.argtypes = [P(TreeArgs), c_void_p]
+    lib.screen_paged_decode_i8.argtypes = [P(TreeArgs), c_void_p]
+    lib.screen_paged_commit.argtypes = [P(CommitArgs), c_void_p]
+    lib.screen_verify_workspace_size.argtypes = [P(VerifyArgs)]
+    lib.screen_verify_workspace_size.restype = c_size_t
+    lib.screen_verify_drafts.argtypes = [P(VerifyArgs), c_void_p]
     lib.screen_dropout_bits.argtypes = [ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32,
                                         ctypes.c_uint32]
     lib.screen_dropout_bits.restype = ctypes.c_uint32
@@ -179,8 +253,10 @@ def load() -> ctypes.CDLL:
     lib.screen_sizeof_args.restype = c_int64
     if lib.screen_version() != ABI_VERSION:
         raise RuntimeError("libscreening_b200.so ABI version mismatch; rebuild it")
-    for i, st in enumerate((FwdArgs, BwdArgs, KVCacheDesc, KVAppendArgs, DecodeArgs,
-                            RowsLinearArgs, XentArgs, RmsNormArgs)):
+    ids = dict(enumerate((FwdArgs, BwdArgs, KVCacheDesc, KVAppendArgs, DecodeArgs,
+                          RowsLinearArgs, XentArgs, RmsNormArgs)))
+    ids.update(enumerate((PagedAppendArgs, PagedReadArgs, TreeArgs, CommitArgs, VerifyArgs), 16))
+    for i, st in ids.items():
         if lib.screen_sizeof_args(i) != ctypes.sizeof(st):
             raise RuntimeError(f"struct {st.__name__} size differs from the C header; rebuild")
     _lib = lib

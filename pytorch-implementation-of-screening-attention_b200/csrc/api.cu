@@ -141,6 +141,11 @@ int64_t screen_sizeof_args(int which) {
     case 5: return (int64_t)sizeof(screen_rows_linear_args);
     case 6: return (int64_t)sizeof(screen_xent_args);
     case 7: return (int64_t)sizeof(screen_rmsnorm_args);
+    case 16: return (int64_t)sizeof(screen_paged_append_args);
+    case 17: return (int64_t)sizeof(screen_paged_read_args);
+    case 18: return (int64_t)sizeof(screen_tree_args);
+    case 19: return (int64_t)sizeof(screen_commit_args);
+    case 20: return (int64_t)sizeof(screen_verify_args);
     default: return -1;
   }
 }

@@ -1,0 +1,280 @@
+"""Attention for a tree of drafted tokens over the paged cache, and the commit
+of its accepted path, against the 64-bit restatement."""
+import math
+
+import pytest
+import torch
+
+from oracle import paged_oracle as po
+from tests.test_paged_int8_gpu import bound
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+def make(ms, B, H, D, ps, T, n, dtype, q8, seed, blocks=None, ring=None):
+    g = torch.Generator().manual_seed(seed)
+    blocks = blocks or (T + n) // ps + 1
+    per = ring or blocks
+    table = torch.randperm(B * per, generator=g).view(B, per)[:, torch.arange(blocks) % per]
+    table = table.to(torch.int32).contiguous().to(DEV)
+    pd = torch.int8 if q8 else dtype
+    kp = torch.zeros(B * per, H, ps, D, dtype=pd, device=DEV)
+    vp = torch.zeros_like(kp)
+    ks = torch.zeros(B * per, H, ps, device=DEV) if q8 else None
+    vs = torch.zeros_like(ks) if q8 else None
+    mean = 0.7 * torch.randn(H, D, generator=g)
+    k = (torch.randn(B, T + n, H, D, generator=g) + mean).to(dtype)
+    v = torch.randn(B, T + n, H, D, generator=g).to(dtype)
+    if T:
+        keep = min(T, per * ps)
+        ms.paged_append(k[:, T - keep:T].to(DEV), v[:, T - keep:T].to(DEV),
+                        torch.full((B,), T - keep, dtype=torch.int32, device=DEV), kp, vp, table, ks, vs)
+    q = (k[:, T - 1:T] if T else k[:, :1]) + 0.8 * torch.randn(B, n, H, D, generator=g)
+    return dict(kp=kp, vp=vp, ks=ks, vs=vs, table=table, q=q.to(dtype), k=k[:, T:], v=v[:, T:], g=g)
+
+
+def tree_parents(B, n, kind, g):
+    if kind == "chain":
+        return None
+    if kind == "star":
+        return torch.full((B, n), -1, dtype=torch.int32)
+    p = torch.stack([torch.stack([torch.randint(-1, max(i, 1), (), generator=g) if i else torch.tensor(-1)
+                                  for i in range(n)]) for _ in range(B)]).to(torch.int32)
+    if kind == "ragged":            # absent nodes, and with them their descendants
+        p[0, n // 2:] = -2
+        if n > 3:
+            p[-1, 2] = 5
+            p[-1, 1] = -9
+    return p
+
+
+def check(ms, c, lens, parents, r, w, dtype, q8, **kw):
+    B, n, H, D = c["q"].shape
+    dev = [None if x is None else x.to(DEV) for x in (c["q"], c["k"], c["v"], lens, parents, r, w)]
+    prefix = [None if x is None else x.cpu().clone() for x in (c["kp"], c["vp"], c["ks"], c["vs"], c["table"])]
+    y = ms.paged_tree_decode(*dev, c["kp"], c["vp"], c["table"], c["ks"], c["vs"], **kw)
+    for b in range(B):
+        lines = po.ancestors(None if parents is None else parents[b], n)
+        here = [i for i in range(n) if lines[i] and lens[b] >= 0]
+        # the nodes' rows as the cache holds them now, each within its rounding
+        held = [po.cache_values(c[x + "p"], c[x + "s"], c["table"], b, [int(lens[b]) + i for i in range(n)])
+                for x in "kv"]
+        for x, got in zip("kv", held):
+            if q8:
+                m, sc = po.int8_rows(c[x][b])
+                row, tol = m.double() * sc[..., None], 2.0**-21
+            else:
+                row, tol = po.unit_rows(c[x][b]), 2.0**-21 + (2.0**-8 if dtype == torch.bfloat16 else 0.0)
+            assert ((got - row)[here].abs() <= tol * row[here].abs() + 1e-12).all()
+        want, sums = po.tree(c["q"][b], held[0], held[1], int(lens[b]), parents, r, w, tuple(prefix), b)
+        err = (y[b].double().cpu() - want).norm(dim=-1)
+        lim = bound(want, sums, r, dtype, q8)
+        assert (err <= lim).all(), (b, float((err - lim).max()))
+        for i in range(n):
+            if not lines[i]:
+                assert (y[b, i] == 0).all()
+    return y
+
+
+SHAPES = [(1, 1, 64, 64, 0, 1), (2, 2, 64, 64, 5, 1), (2, 2, 64, 64, 130, 5), (3, 2, 64, 16, 200, 16),
+          (2, 3, 16, 8, 61, 17), (2, 2, 32, 24, 150, 33), (1, 2, 128, 100, 260, 64), (2, 2, 64, 64, 300, 64),
+          (1, 2, 128, 64, 90, 20), (1, 2, 64, 64, 64, 31), (1, 1, 32, 16, 1, 64), (1, 2, 16, 64, 90, 40)]
+
+
+@pytest.mark.parametrize("kind", ["chain", "random", "ragged"])
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True),
+                                      (torch.float32, False), (torch.float32, True)])
+@pytest.mark.parametrize("B,H,D,ps,T,n", SHAPES)
+def test_tree(ms, B, H, D, ps, T, n, dtype, q8, kind):
+    c = make(ms, B, H, D, ps, T, n, dtype, q8, 31 * n + T)
+    lens = torch.tensor([max(0, T - 3 * b) for b in range(B)], dtype=torch.int32)
+    r, w = torch.linspace(1.05, 1.8, H), torch.linspace(T + 30.0, max(3.5, T / 5), H)
+    check(ms, c, lens, tree_parents(B, n, kind, c["g"]), r, w, dtype, q8)
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True),
+                                      (torch.float32, False), (torch.float32, True)])
+@pytest.mark.parametrize("splits", [1, 2, 7, 40])
+def test_splits_agree(ms, dtype, q8, splits):
+    """Any number of splits, and any hint of the window, gives the same rows to
+    the order of the sums; twice the same call gives the same bits."""
+    c = make(ms, 2, 2, 64, 16, 500, 9, dtype, q8, 5)
+    lens = torch.tensor([500, 444], dtype=torch.int32)
+    parents = tree_parents(2, 9, "random", c["g"])
+    r, w = torch.tensor([1.1, 1.4]), torch.tensor([600.0, 90.0])
+    y = check(ms, c, lens, parents, r, w, dtype, q8, num_splits=splits, max_window=3)
+    z = check(ms, c, lens, parents, r, w, dtype, q8, num_splits=splits, max_window=3)
+    assert torch.equal(y, z)
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)])
+def test_paths_equal_tokens_one_by_one(ms, dtype, q8):
+    """A chain of drafts gives what single-token steps give, and leaves the same
+    cache behind, over a ring that wraps."""
+    B, H, D, ps, T, n = 2, 2, 64, 16, 90, 7
+    w = torch.tensor([40.0, 12.5])
+    per = math.ceil((40 + n) / ps) + 1
+    r = torch.tensor([1.1, 1.5])
+    a = make(ms, B, H, D, ps, T, n, dtype, q8, 9, ring=per)
+    b = make(ms, B, H, D, ps, T, n, dtype, q8, 9, ring=per)
+    lens = torch.full((B,), T, dtype=torch.int32, device=DEV)
+    args = (r.to(DEV), w.to(DEV))
+    y = ms.paged_tree_decode(a["q"].to(DEV), a["k"].to(DEV), a["v"].to(DEV), lens, None, *args,
+                             a["kp"], a["vp"], a["table"], a["ks"], a["vs"])
+    for i in range(n):
+        ms.paged_append(b["k"][:, i:i + 1].to(DEV), b["v"][:, i:i + 1].to(DEV), lens + i, b["kp"], b["vp"],
+                        b["table"], b["ks"], b["vs"])
+        z = ms.paged_decode(b["q"][:, i].to(DEV), lens + i + 1, *args, b["kp"], b["vp"], b["table"],
+                            b["ks"], b["vs"])
+        # bf16: both sides round the output (2^-8 each); the tree also rounds alpha
+        # (2^-8 of sums with little cancellation here)
+        tol = 2.0**-6 if dtype == torch.bfloat16 else 2.0**-17
+        assert ((y[:, i] - z).float().norm(dim=-1) <= tol * z.float().norm(dim=-1) + 1e-6).all(), i
+    for x in ("kp", "vp", "ks", "vs"):
+        if a[x] is not None:
+            assert torch.equal(a[x], b[x])
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)])
+def test_non_finite_rows_stay_where_they_are_seen(ms, dtype, q8):
+    B, H, D, ps, T, n = 1, 2, 64, 16, 70, 6
+    c = make(ms, B, H, D, ps, T, n, dtype, q8, 12)
+    parents = torch.tensor([[-1, 0, 0, 1, 2, -1]], dtype=torch.int32, device=DEV)
+    lens = torch.full((1,), T, dtype=torch.int32, device=DEV)
+    r, w = torch.full((H,), 1.01, device=DEV), torch.full((H,), 60.0, device=DEV)
+    q, k, v = (c[x].to(DEV) for x in "qkv")
+    q, k = q.abs() + 0.1, k.abs() + 0.1             # every pair is over the trim
+
+    def run(v, k=k, q=q):
+        return ms.paged_tree_decode(q, k, v, lens, parents, r, w, c["kp"], c["vp"], c["table"], c["ks"], c["vs"])
+
+    good = run(v)
+    assert good.isfinite().all()
+    for bad in (math.nan, math.inf, -math.inf):
+        vv = v.clone()
+        vv[0, 1, 0, 3] = bad                         # node 1, head 0: seen by nodes 1 and 3
+        y = run(vv)
+        assert y[0, [1, 3], 0].isnan().all()
+        keep = torch.ones(n, H, dtype=torch.bool)
+        keep[[1, 3], 0] = False
+        assert torch.equal(y[0][keep], good[0][keep])
+    kk = k.clone()
+    kk[0, 2, 1, 0] = math.nan                        # a key that is not seen by anyone
+    y = run(v, k=kk)
+    assert y.isfinite().all() and torch.equal(y[0, :, 0], good[0, :, 0])
+    assert torch.equal(y[0, [0, 1, 3, 5], 1], good[0, [0, 1, 3, 5], 1])
+    qq = q.clone()
+    qq[0, 4] = math.nan                              # a query that sees nothing
+    y = run(v, q=qq)
+    assert (y[0, 4] == 0).all() and torch.equal(y[0, :4], good[0, :4])
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)])
+def test_absent_nodes_and_empty_places_write_nothing(ms, dtype, q8):
+    B, H, D, ps, T, n = 3, 2, 64, 16, 40, 8
+    c = make(ms, B, H, D, ps, T, n, dtype, q8, 21)
+    parents = torch.tensor([[-1, 0, -2, 2, 1, -1, 9, 6]] * B, dtype=torch.int32, device=DEV)
+    lens = torch.tensor([T, -1, T - 7], dtype=torch.int32, device=DEV)
+    k = c["k"].to(DEV)
+    k[:, 2] = math.nan
+    before = [None if c[x] is None else c[x].clone() for x in ("kp", "vp", "ks", "vs")]
+    r, w = torch.full((H,), 1.2, device=DEV), torch.full((H,), 30.0, device=DEV)
+    y = ms.paged_tree_decode(c["q"].to(DEV), k, c["v"].to(DEV), lens, parents, r, w, c["kp"], c["vp"], c["table"],
+                             c["ks"], c["vs"])
+    assert (y[1] == 0).all() and (y[:, [2, 3, 6, 7]] == 0).all() and y.isfinite().all()
+    wrote = {(b, i) for b, l in ((0, T), (2, T - 7)) for i in (0, 1, 4, 5)}
+    allowed = torch.zeros(c["kp"].shape[0], ps, dtype=torch.bool)
+    for b, i in wrote:
+        p = int(lens[b]) + i
+        allowed[int(c["table"][b, p // ps]), p % ps] = True
+    for x, old in zip(("kp", "vp"), before):
+        diff = (c[x] != old).any(-1).any(1).cpu()
+        assert not (diff & ~allowed).any() and diff.any()
+
+
+def test_nodes_past_the_table_are_not_seen(ms):
+    c = make(ms, 1, 2, 64, 16, 30, 6, torch.bfloat16, False, 2, blocks=2)
+    lens = torch.full((1,), 30, dtype=torch.int32, device=DEV)       # rows 32 .. 35 have no place
+    r, w = torch.full((2,), 1.05, device=DEV), torch.full((2,), 64.0, device=DEV)
+    y = ms.paged_tree_decode(c["q"].to(DEV), c["k"].to(DEV), c["v"].to(DEV), lens, None, r, w, c["kp"], c["vp"],
+                             c["table"])
+    assert y.isfinite().all() and (y[0, :2] != 0).any()
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.float32, False), (torch.bfloat16, True)])
+@pytest.mark.parametrize("L,B,n,H,D,ps", [(1, 1, 1, 1, 16, 8), (3, 2, 5, 2, 64, 16), (2, 3, 64, 2, 128, 24)])
+def test_commit(ms, L, B, n, H, D, ps, dtype, q8):
+    g = torch.Generator().manual_seed(n)
+    T = 20
+    blocks = (T + n) // ps + 2
+    table = torch.randperm(B * blocks, generator=g).view(B, blocks).to(torch.int32)
+    shape = (L, B * blocks, H, ps, D)
+    kp = torch.randint(-127, 128, shape, generator=g).to(torch.int8) if q8 else torch.randn(shape, generator=g).to(dtype)
+    vp = kp.flip(0).clone().contiguous()
+    ks = torch.rand(shape[:-1], generator=g) if q8 else None
+    vs = torch.rand(shape[:-1], generator=g) if q8 else None
+    lens = torch.tensor([T - b for b in range(B)], dtype=torch.int32)
+    counts = torch.randint(0, n + 1, (B,), generator=g).to(torch.int32)
+    counts[0] = n
+    path = torch.stack([torch.randperm(n, generator=g).sort().values if b == 0 else torch.randperm(n, generator=g)
+                        for b in range(B)]).to(torch.int32)          # any order is allowed
+    if n > 4:
+        path[-1, 1] = -1
+        path[-1, 3] = n + 4
+        counts[-1] = n + 9                                            # read as n
+    lens[-1] = -1 if B > 2 else lens[-1]
+    want = [None if x is None else x.clone() for x in (kp, vp, ks, vs)]
+    for b in range(B):
+        if lens[b] < 0:
+            continue
+        for x, old in zip(want, (kp, vp, ks, vs)):
+            if x is None:
+                continue
+            for i in range(min(int(counts[b]), n)):
+                p = int(path[b, i])
+                if not 0 <= p < n:
+                    continue
+                f, t = int(lens[b]) + p, int(lens[b]) + i
+                x[:, table[b, t // ps], :, t % ps] = old[:, table[b, f // ps], :, f % ps]
+    dev = [None if x is None else x.to(DEV) for x in (kp, vp, table, ks, vs)]
+    ms.paged_commit(lens.to(DEV), path.to(DEV), counts.to(DEV), *dev)
+    for x, y in zip((dev[0], dev[1], dev[3], dev[4]), want):
+        assert x is None or torch.equal(x.cpu(), y)
+    if L == 1:                                                        # without the layer dimension
+        dev2 = [None if x is None else (x[0] if x.dim() > 2 else x).to(DEV).contiguous() for x in (kp, vp, table, ks, vs)]
+        ms.paged_commit(lens.to(DEV), path.to(DEV), counts.to(DEV), *dev2)
+        assert torch.equal(dev2[0].cpu(), want[0][0])
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_captured_and_on_two_streams(ms, q8):
+    """Two captured graphs replayed on two streams, and an eager call between
+    them, share nothing."""
+    cs = [make(ms, 2, 2, 64, 16, 400, 9, torch.bfloat16, q8, s) for s in (3, 4)]
+    lens = torch.tensor([400, 380], dtype=torch.int32, device=DEV)
+    r, w = torch.tensor([1.1, 1.4], device=DEV), torch.tensor([600.0, 90.0], device=DEV)
+
+    def run(c):
+        return ms.paged_tree_decode(c["dq"], c["dk"], c["dv"], lens, None, r, w, c["kp"], c["vp"], c["table"], c["ks"],
+                                    c["vs"], num_splits=4)
+
+    for c in cs:
+        c["dq"], c["dk"], c["dv"] = (c[x].to(DEV) for x in "qkv")
+    want = [run(c).clone() for c in cs]
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for c in cs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run(c))
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    eager = run(cs[0])
+    torch.cuda.synchronize()
+    for o, x in zip(outs, want):
+        assert torch.equal(o, x)
+    assert torch.equal(eager, want[0])

@@ -1,0 +1,183 @@
+"""Verification of drafted tokens against the 64-bit restatement: whole
+numbers, equal."""
+import math
+
+import pytest
+import torch
+
+from oracle import paged_oracle as po
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+def parents_of(B, n, kind, g):
+    if kind == "chain":
+        return None
+    if kind == "star":
+        return torch.full((B, n), -1, dtype=torch.int32)
+    p = torch.stack([torch.stack([torch.randint(-1, i, (), generator=g) if i else torch.tensor(-1) for i in range(n)])
+                     for _ in range(B)]).to(torch.int32)
+    if kind == "ragged":
+        p[0, n // 2:] = -2
+        p[-1, n - 1] = n + 3
+    return p
+
+
+def case(B, n, V, kind, drawn, temp, dtype, seed, sharp=2.0):
+    g = torch.Generator().manual_seed(seed)
+    logits = torch.randn(B, n + 1, V, generator=g) * sharp
+    parents = parents_of(B, n, kind, g)
+    row = (torch.arange(n).expand(B, n) if parents is None else parents.long() + 1).clamp(0, max(n - 1, 0))
+    dl = None
+    src = logits
+    if drawn:
+        dl = (logits[:, :n] + 0.8 * torch.randn(B, n, V, generator=g)).to(dtype)
+        src = dl.float()
+    gumbel = -torch.log(-torch.log(torch.rand(B, n, V, generator=g).clamp(1e-6, 1 - 1e-6)))
+    pick = src[:, :n] if n else src[:, :0]
+    tokens = (pick.float().gather(1, row[..., None].expand(B, n, V)) / max(temp, 0.05) + gumbel).argmax(-1) \
+        if n else torch.zeros(B, 0, dtype=torch.long)
+    return dict(logits=logits.to(dtype), tokens=tokens, parents=parents, uniforms=torch.rand(B, n + 1, generator=g),
+                draft_logits=dl)
+
+
+def check(ms, c, temp, **kw):
+    dev = {k: None if x is None else x.to(DEV) for k, x in c.items()}
+    out, path, counts = ms.verify_drafts(dev["logits"], dev["tokens"], dev["parents"], dev["uniforms"],
+                                         draft_logits=dev["draft_logits"], temperature=temp)
+    B, n = c["tokens"].shape
+    assert out.shape == (B, n + 1) and path.shape == (B, n) and counts.shape == (B,)
+    total = 0
+    for b in range(B):
+        t = float(temp[b]) if isinstance(temp, torch.Tensor) else temp
+        want = po.verify(c["logits"][b], c["tokens"][b], None if c["parents"] is None else c["parents"][b],
+                         c["uniforms"][b], None if c["draft_logits"] is None else c["draft_logits"][b], t)
+        a = int(counts[b])
+        total += a
+        assert a == want[2] and path[b].tolist() == want[1] + [-1] * (n - a), (b, want)
+        assert out[b].tolist() == want[0] + [-1] * (n - a), (b, want)
+    return total
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("kind", ["chain", "star", "random", "ragged"])
+@pytest.mark.parametrize("B,n,V,temp", [(1, 1, 5, 1.0), (3, 4, 1000, 0.7), (2, 7, 50257, 1.0), (4, 16, 999, 1.3),
+                                        (2, 64, 2049, 0.9), (3, 5, 129, 0.0)])
+def test_against_the_restatement(ms, B, n, V, temp, kind, drawn, dtype):
+    total = sum(check(ms, case(B, n, V, kind, drawn, temp, dtype, 17 * n + V + s), temp) for s in range(3))
+    if n >= 4 and drawn and kind == "chain":
+        assert total > 0                                 # some were accepted
+
+
+def test_lazy_rows_equal_up_front_rows(ms):
+    """Above 48 MB of logits rows are read as the walk reaches them: a batch of
+    copies of a small case gives each copy the small case's answer."""
+    c = case(2, 31, 50257, "random", True, 1.0, torch.bfloat16, 5)
+    small = ms.verify_drafts(*(c[k].to(DEV) for k in ("logits", "tokens", "parents", "uniforms")),
+                             draft_logits=c["draft_logits"].to(DEV))
+    big = {k: x.to(DEV).repeat_interleave(8, 0) for k, x in c.items()}
+    assert (big["logits"].numel() + big["draft_logits"].numel()) * 2 > 48 << 20
+    out = ms.verify_drafts(big["logits"], big["tokens"], big["parents"], big["uniforms"],
+                           draft_logits=big["draft_logits"])
+    for x, y in zip(out, small):
+        assert torch.equal(x, y.repeat_interleave(8, 0))
+    check(ms, c, 1.0)
+
+
+def test_no_drafts_is_plain_sampling(ms):
+    check(ms, case(5, 0, 777, "chain", False, 0.8, torch.float32, 3), 0.8)
+    check(ms, case(5, 0, 777, "chain", True, 0.8, torch.float32, 3), 0.8)
+
+
+def test_temperatures_per_sequence_and_strided_rows(ms):
+    c = case(4, 6, 501, "random", True, 1.0, torch.float32, 8)
+    temps = torch.tensor([0.0, 0.5, 1.0, 40.0])
+    check(ms, c, temps.to(DEV))
+    # rows of an odd stride, and a view of wider rows
+    wide = torch.full((4, 7, 512), 50.0)
+    wide[..., :501] = c["logits"]
+    dev = {k: x.to(DEV) for k, x in c.items()}
+    a = ms.verify_drafts(wide.to(DEV)[..., :501], dev["tokens"], dev["parents"], dev["uniforms"],
+                         draft_logits=dev["draft_logits"])
+    b = ms.verify_drafts(dev["logits"], dev["tokens"], dev["parents"], dev["uniforms"],
+                         draft_logits=dev["draft_logits"])
+    t = ms.verify_drafts(dev["logits"].transpose(1, 2).contiguous().transpose(1, 2),
+                         dev["tokens"].t().contiguous().t(), dev["parents"].t().contiguous().t(),
+                         dev["uniforms"].t().contiguous().t(), draft_logits=dev["draft_logits"])
+    for x, y, z in zip(a, b, t):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+def test_masked_and_unusable_rows(ms):
+    """-inf entries have probability 0; rows without a finite maximum, with +inf
+    or NaN accept nothing; tokens outside the vocabulary are never accepted."""
+    for drawn in (False, True):
+        c = case(8, 3, 300, "chain", drawn, 1.0, torch.float32, 4, sharp=0.5)
+        c["uniforms"][:, :3] = 0.0                         # whatever can be accepted is
+        c["logits"][0, 0] = -math.inf
+        c["logits"][1, 1, 7] = math.nan
+        c["logits"][2, 0, 5] = math.inf
+        c["logits"][3, 0, 100:] = -math.inf
+        c["logits"][4, 0, int(c["tokens"][4, 0])] = -math.inf
+        c["tokens"][5, 1] = 300
+        c["tokens"][6, 0] = -4
+        if drawn:
+            c["draft_logits"][7, 0] = -math.inf
+        c["logits"][7, 0, :299] = -math.inf                # one token left
+        check(ms, c, 1.0)
+        dev = {k: None if x is None else x.to(DEV) for k, x in c.items()}
+        out, _, counts = ms.verify_drafts(dev["logits"], dev["tokens"], None, dev["uniforms"],
+                                          draft_logits=dev["draft_logits"])
+        assert out[0, 0] == -1 and out[2, 0] == -1 and counts[6] == 0
+        check(ms, c, 0.0)
+
+
+def test_same_model_accepts_everything(ms):
+    c = case(3, 6, 4001, "chain", True, 1.0, torch.bfloat16, 6)
+    c["draft_logits"] = c["logits"][:, :6].clone()
+    assert check(ms, c, 1.0) == 18
+
+
+def test_uniforms_at_the_ends(ms):
+    for u in (0.0, 1.0 - 2.0**-24, 1.0):
+        c = case(4, 2, 1000, "chain", True, 1.0, torch.bfloat16, 11)
+        c["uniforms"].fill_(u)
+        check(ms, c, 1.0)
+        c["logits"][:, :, 900:] = -math.inf                # the last weighted index is not the last
+        check(ms, c, 1.0)
+
+
+def test_samples_follow_the_target(ms):
+    """20000 independent chains of one draft: the first token is distributed as
+    the target's, whatever the drafting model (chi-square, 11 degrees)."""
+    N, V = 20000, 12
+    g = torch.Generator(device=DEV).manual_seed(0)
+    lt = torch.randn(1, 2, V, device=DEV, generator=g)
+    ld = torch.randn(1, 1, V, device=DEV, generator=g)
+    tok = torch.multinomial(ld[0, 0].softmax(-1), N, replacement=True, generator=g)[:, None]
+    u = torch.rand(N, 2, device=DEV, generator=g)
+    out, _, counts = ms.verify_drafts(lt.expand(N, 2, V), tok, None, u, draft_logits=ld.expand(N, 1, V))
+    seen = torch.bincount(out[:, 0], minlength=V).double().cpu()
+    want = lt[0, 0].double().softmax(-1).cpu() * N
+    assert 0 < int(counts.sum()) < N
+    assert float(((seen - want) ** 2 / want).sum()) < 31.3   # exceeded once in 1000 by a fair draw
+
+
+def test_captured(ms):
+    c = case(3, 5, 5003, "random", True, 1.0, torch.bfloat16, 2)
+    dev = {k: x.to(DEV) for k, x in c.items()}
+
+    def run():
+        return ms.verify_drafts(dev["logits"], dev["tokens"], dev["parents"], dev["uniforms"],
+                                draft_logits=dev["draft_logits"])
+
+    want = [x.clone() for x in run()]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    for _ in range(5):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(out, want))
