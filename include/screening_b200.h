@@ -297,12 +297,10 @@ typedef struct screen_tree_args {
   int32_t dtype;                 /* of q, k, v, y                             */
   int32_t cache_dtype;           /* = dtype, or SCREEN_I8                     */
   int32_t B, H, D, n;            /* n <= SCREEN_TREE_MAX_NODES nodes          */
-  int32_t num_splits;            /* runs the key axis is cut into; >= 1       */
-  int32_t max_window;            /* keys a query is expected to see (<= 0:    */
-                                 /*   the table's length); sets the share of  */
-                                 /*   a split, not what is seen               */
+  int32_t num_ctas;              /* 1: one CTA per (sequence, head); more:    */
+                                 /*   all key tiles are shared out over that  */
+                                 /*   many CTAs, a second pass adds the parts */
   float eps;
-  int32_t _pad0;
   const void* q; int64_t q_sb, q_st;   /* raw (B,n,H,D)                       */
   const void* k; int64_t k_sb, k_st;   /* raw rows of the nodes, or NULL:     */
   const void* v; int64_t v_sb, v_st;   /*   they are in the cache already     */

@@ -137,8 +137,7 @@ class PagedReadArgs(ctypes.Structure):
 class TreeArgs(ctypes.Structure):
     _fields_ = [
         ("dtype", c_int32), ("cache_dtype", c_int32), ("B", c_int32), ("H", c_int32),
-        ("D", c_int32), ("n", c_int32), ("num_splits", c_int32), ("max_window", c_int32),
-        ("eps", c_float), ("_pad0", c_int32),
+        ("D", c_int32), ("n", c_int32), ("num_ctas", c_int32), ("eps", c_float),
         ("q", c_void_p), ("q_sb", c_int64), ("q_st", c_int64),
         ("k", c_void_p), ("k_sb", c_int64), ("k_st", c_int64),
         ("v", c_void_p), ("v_sb", c_int64), ("v_st", c_int64),

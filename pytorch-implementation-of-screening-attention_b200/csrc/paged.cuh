@@ -8,12 +8,12 @@ void paged_append8(const screen_paged_append_args& a, cudaStream_t s);
 void paged_read(const screen_paged_read_args& a, cudaStream_t s);
 void commit(const screen_commit_args& a, cudaStream_t s);
 
-// Positions are cut into tiles of kTreeTile keys, a split owns a run of them.
+// Positions are cut into tiles of kTreeTile keys.
 constexpr int kTreeTile = 64;
 struct TreeParams {
   screen_tree_args a;
-  int per;        // tiles a split owns at least (see tree_range)
   int lens_off;   // added to a.lens (decode: -1, the query is the newest cached token)
+  int part_off;   // floats of the workspace before the partial sums
 };
 void tree_bf16(const TreeParams& p, float* part, cudaStream_t s);
 void tree_i8(const TreeParams& p, float* part, cudaStream_t s);

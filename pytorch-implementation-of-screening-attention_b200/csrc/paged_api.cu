@@ -21,14 +21,15 @@ int cache_ok(const screen_kv_cache& c, int cache_dtype, const float* ks, const f
   if (!al16(c.k_pages) || !al16(c.v_pages) || !al4(ks) || !al4(vs)) return SCREEN_ERR_ALIGNMENT;
   return SCREEN_OK;
 }
-// grid.y = B * H
-bool grid_ok(long long bh) { return bh <= 65535; }
+// floats of the tree workspace before the partial sums: two ints per segment
+long long part_off(const screen_tree_args* a) { return ((long long)a->B * a->H * 2 + 3) & ~3ll; }
 
 int tree_checks(const screen_tree_args* a) {
   if (!act_ok(a->dtype)) return SCREEN_ERR_DTYPE;
   if (a->cache_dtype != a->dtype && a->cache_dtype != SCREEN_I8) return SCREEN_ERR_DTYPE;
   if (!dim_ok(a->D)) return SCREEN_ERR_HEAD_DIM;
-  if (a->B < 0 || a->H < 0 || a->n < 0 || a->n > SCREEN_TREE_MAX_NODES || a->num_splits < 1)
+  if (a->B < 0 || a->H < 0 || a->n < 0 || a->n > SCREEN_TREE_MAX_NODES || a->num_ctas < 1 ||
+      a->num_ctas > 65535)
     return SCREEN_ERR_INVALID_ARG;
   return SCREEN_OK;
 }
@@ -36,7 +37,7 @@ int tree_run(const screen_tree_args* a, int lens_off, cudaStream_t s) {
   if ((long long)a->B * a->H * a->n == 0) return SCREEN_OK;
   if (!a->q || !a->lens || !a->r || !a->w || !a->y || (!a->k) != (!a->v))
     return SCREEN_ERR_INVALID_ARG;
-  if (!grid_ok((long long)a->B * a->H)) return SCREEN_ERR_UNSUPPORTED;
+  if ((long long)a->B * a->H > (1 << 28)) return SCREEN_ERR_UNSUPPORTED;
   int st = cache_ok(a->cache, a->cache_dtype, a->k_scales, a->v_scales);
   if (st) return st;
   if (!raw_ok(a->q, a->q_sb, a->q_st) || !al16(a->y)) return SCREEN_ERR_ALIGNMENT;
@@ -45,12 +46,7 @@ int tree_run(const screen_tree_args* a, int lens_off, cudaStream_t s) {
   const size_t need = screen_tree_workspace_size(a);
   if (need && (!a->workspace || a->workspace_bytes < need)) return SCREEN_ERR_WORKSPACE;
   if (need && !al16(a->workspace)) return SCREEN_ERR_ALIGNMENT;
-  // the widest head's tiles over the splits
-  const long long table = (long long)a->cache.max_blocks * a->cache.page_size;
-  long long keys = a->max_window > 0 && a->max_window < table ? a->max_window : table;
-  keys += a->n;
-  const long long tiles = keys / kTreeTile + 2;
-  TreeParams p{*a, (int)((tiles + a->num_splits - 1) / a->num_splits), lens_off};
+  TreeParams p{*a, lens_off, (int)part_off(a)};
   float* part = reinterpret_cast<float*>(a->workspace);
   if (a->cache_dtype == SCREEN_I8) {
     if (a->dtype == SCREEN_F32) tree_i8_f32(p, part, s);
@@ -61,7 +57,7 @@ int tree_run(const screen_tree_args* a, int lens_off, cudaStream_t s) {
     tree_bf16(p, part, s);
   }
   st = check_launch();
-  if (st || a->num_splits == 1) return st;
+  if (st || a->num_ctas == 1) return st;
   tree_finish(p, part, s);
   return check_launch();
 }
@@ -100,8 +96,9 @@ int screen_paged_read(const screen_paged_read_args* a, screen_stream_t stream) {
 }
 
 size_t screen_tree_workspace_size(const screen_tree_args* a) {
-  if (!a || tree_checks(a) || a->num_splits == 1) return 0;
-  return round_up((size_t)a->B * a->H * a->num_splits * a->n * a->D * sizeof(float));
+  if (!a || tree_checks(a) || a->num_ctas == 1) return 0;
+  // a slot per (CTA, segment) pair along the tile list
+  return round_up((part_off(a) + ((size_t)a->B * a->H + a->num_ctas) * a->n * a->D) * sizeof(float));
 }
 
 int screen_tree_decode(const screen_tree_args* a, screen_stream_t stream) {

@@ -10,22 +10,19 @@
 // There is no softmax normaliser, so partial sums over runs of keys simply add.
 //
 // Work: 4 D flops per (query, key) against 2 row reads per key shared by all n
-// queries of a head.  For the n here the reads of the keys are what a pass
-// cannot do without (n = 64, D = 64, int8: 120 flops a byte), so the kernel is
-// built around one pass over the pages: a CTA owns a run of 64-key tiles of one
-// (sequence, head) and keeps every query of the tree in registers.
+// queries of a head.  The reads of the keys are what a pass cannot do without,
+// so the kernels are built around one pass over the pages.
 //
-//  * tiles are copied with cp.async (16 bytes, XOR-swizzled rows, zero fill for
-//    keys outside the window or the table) into a ring of shared-memory stages;
-//    pages of any size work because every row has its own address, looked up a
-//    stage ahead of its copies;
-//  * S and alpha V run on warp-level MMAs (m16n8k16, queries on the 16 rows):
-//    with one to 64 query rows a 128-row tcgen05 tile would be mostly padding,
-//    and the score fragment is directly the A operand of alpha V;
-//  * a group of 16 keys whose scores all fall under the trim skips the mask and
-//    the alpha V product;
-//  * the mask is cos(pi (c_j - d_i) / w) = cos cos + sin sin with one pair per
-//    key (c_j: position minus lens, or the node's depth) and one per query.
+// Sharing out the keys.  Positions are cut into 64-key tiles; the tiles of all
+// (sequence, head) segments, one after another, form one list that is cut into
+// equal runs, a CTA each.  Heads have windows of very different lengths (2 to
+// thousands of keys in one layer), so a fixed number of splits per head would
+// leave most CTAs idle while the widest head's work; the list needs no host
+// knowledge of lengths or windows.  A CTA that owns only a part of a segment
+// leaves its sum in workspace slot (CTA + segment), which no other pair shares
+// because both grow along the list, and tree_finish_kernel adds a segment's
+// slots in order.  With few tiles a segment goes to one CTA and no second launch
+// follows.
 #pragma once
 #include "kv_rows.cuh"
 #include "paged.cuh"
@@ -38,19 +35,20 @@ constexpr int kThreads = 128;
 constexpr int kMaxN = SCREEN_TREE_MAX_NODES;
 constexpr int kNoKey = -2000000000;   // c of a key that nothing sees
 
-// Tiles [t0, t1] that sequence b, head h reads, and the tiles one split owns.
+// Tiles [t0, t0 + nt) that sequence b, head h reads.
 struct Range {
   long long lens, first;  // first: oldest key any node sees
-  int t0, nt, per, used;  // used: splits that own a tile
-  int dmax;
+  int t0, nt, dmax;       // nt >= 1, a dummy tile for an empty place
+  bool any;
 };
 __device__ __forceinline__ Range tree_range(const TreeParams& p, int b, int h) {
   Range g;
   g.lens = (long long)p.a.lens[b] + p.lens_off;
   g.dmax = window_dmax(p.a.w[h]);
-  if (g.lens < 0) {  // an empty place in the batch
-    g.t0 = g.nt = g.used = 0;
-    g.per = 1;
+  g.any = g.lens >= 0;
+  if (!g.any) {  // an empty place in the batch
+    g.t0 = 0;
+    g.nt = 1;
     g.first = 0;
     return g;
   }
@@ -58,12 +56,115 @@ __device__ __forceinline__ Range tree_range(const TreeParams& p, int b, int h) {
   if (g.first < 0) g.first = 0;
   g.t0 = (int)(g.first / kTile);
   g.nt = (int)((g.lens + p.a.n - 1) / kTile) - g.t0 + 1;
-  // the host's tiles per split gives every CTA the same work across heads of
-  // different windows; a window wider than the host was told still fits
-  const int least = (g.nt + p.a.num_splits - 1) / p.a.num_splits;
-  g.per = p.per > least ? p.per : least;
-  g.used = (g.nt + g.per - 1) / g.per;
   return g;
+}
+
+// A CTA's run of the tile list, segment by segment.
+struct Share {
+  long long pos, end, start;   // next tile, end of the run, first tile of `seg`
+  long long total;
+  int ctas;                    // CTAs that have a run
+  int seg;
+};
+// Slots of the partial sums of each segment: CTAs first .. last, none if the
+// segment's rows were written by the CTA that owned all of it.
+struct SegSlots {
+  int first, last;
+};
+constexpr int kMinTiles = 4;   // a run is at least this long
+__device__ __forceinline__ long long share_begin(const Share& s, int cta) {
+  return s.total * cta / s.ctas;
+}
+// All threads of the CTA; false if it has nothing to do.
+__device__ __forceinline__ bool share_init(const TreeParams& p, Share& s) {
+  const int segs = p.a.B * p.a.H;
+  if (p.a.num_ctas == 1) {     // one CTA per segment
+    s.seg = blockIdx.x;
+    s.start = s.pos = 0;
+    s.ctas = 0;
+    return true;
+  }
+  __shared__ long long warp_s[kThreads / 32];
+  __shared__ long long start_s;
+  __shared__ int seg_s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int each = (segs + kThreads - 1) / kThreads;
+  long long mine = 0;
+  for (int j = tid * each; j < (tid + 1) * each && j < segs; ++j)
+    mine += tree_range(p, j / p.a.H, j % p.a.H).nt;
+  long long inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) warp_s[warp] = inc;
+  __syncthreads();
+  long long before = inc - mine;
+  s.total = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) {
+    if (i < warp) before += warp_s[i];
+    s.total += warp_s[i];
+  }
+  const long long most = (s.total + kMinTiles - 1) / kMinTiles;
+  s.ctas = (long long)gridDim.x < most ? (int)gridDim.x : (int)most;
+  if ((int)blockIdx.x >= s.ctas) return false;
+  s.pos = share_begin(s, blockIdx.x);
+  s.end = share_begin(s, blockIdx.x + 1);
+  if (s.pos >= before && s.pos < before + mine) {   // this thread's segments hold it
+    int j = tid * each;
+    long long at = before;
+    while (true) {
+      const int nt = tree_range(p, j / p.a.H, j % p.a.H).nt;
+      if (s.pos < at + nt) break;
+      at += nt;
+      ++j;
+    }
+    seg_s = j;
+    start_s = at;
+  }
+  __syncthreads();
+  s.seg = seg_s;
+  s.start = start_s;
+  return true;
+}
+// Next piece: tiles [c0, c1] of segment s.seg.  False at the end of the run.
+__device__ __forceinline__ bool share_next(const TreeParams& p, Share& s, Range& g, int& c0,
+                                           int& c1, bool& whole, SegSlots* slots) {
+  if (s.ctas == 0) {
+    if (s.pos) return false;
+    g = tree_range(p, s.seg / p.a.H, s.seg % p.a.H);
+    c0 = g.t0;
+    c1 = g.t0 + g.nt - 1;
+    whole = true;
+    s.pos = 1;
+    return true;
+  }
+  if (s.pos >= s.end) return false;
+  if (s.pos >= s.start) {
+    g = tree_range(p, s.seg / p.a.H, s.seg % p.a.H);
+    while (s.pos >= s.start + g.nt) {   // the previous piece ended its segment
+      s.start += g.nt;
+      ++s.seg;
+      g = tree_range(p, s.seg / p.a.H, s.seg % p.a.H);
+    }
+  }
+  const long long stop = s.end < s.start + g.nt ? s.end : s.start + g.nt;
+  c0 = g.t0 + (int)(s.pos - s.start);
+  c1 = g.t0 + (int)(stop - s.start) - 1;
+  whole = s.pos == s.start && stop == s.start + g.nt;
+  if (s.pos == s.start && threadIdx.x == 0) {
+    SegSlots q{0, -1};
+    if (!whole) {
+      q.first = blockIdx.x;
+      // the last CTA whose run begins at or before the segment's last tile
+      q.last = (int)(((s.start + g.nt) * s.ctas - 1) / s.total);
+    }
+    slots[s.seg] = q;
+  }
+  s.pos = stop;
+  return true;
 }
 
 // Ancestor masks, depths and presence of the n nodes of sequence b, by warp 0:
@@ -157,6 +258,10 @@ __device__ __forceinline__ void store_row(const screen_tree_args& a, int b, int 
 #pragma unroll
   for (int e = 0; e < PER; ++e)
     if (lane + 32 * e < D) y[lane + 32 * e] = from_f<TA>(present ? o[e] * g : 0.f);
+}
+
+inline dim3 tree_grid(const TreeParams& p) {
+  return dim3(p.a.num_ctas == 1 ? p.a.B * p.a.H : p.a.num_ctas);
 }
 
 }  // namespace tree

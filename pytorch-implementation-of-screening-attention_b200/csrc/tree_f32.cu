@@ -11,7 +11,7 @@ namespace {
 constexpr int kKeys = 32;
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) tree_f32_kernel(TreeParams p, float* __restrict__ part) {
+__global__ void __launch_bounds__(kThreads) tree_f32_kernel(TreeParams p, float* __restrict__ ws) {
   constexpr int LD = D + 4;                        // rows of 16-byte pieces on distinct banks
   constexpr int QG = kThreads / D < 1 ? 1 : kThreads / D;  // query groups in alpha V
   constexpr int PQ = (kMaxN + QG - 1) / QG;
@@ -27,18 +27,22 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(TreeParams p, float*
   pdl_trigger();
   const screen_tree_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int bh = blockIdx.y, b = bh / a.H, h = bh % a.H, split = blockIdx.x;
-  const Range rg = tree_range(p, b, h);
-  const int c0 = rg.t0 + split * rg.per;
-  int c1 = c0 + rg.per - 1;
-  if (c1 > rg.t0 + rg.nt - 1) c1 = rg.t0 + rg.nt - 1;
-  if (split >= (rg.used > 0 ? rg.used : 1)) return;
+  const int n = a.n;
+  SegSlots* slots = reinterpret_cast<SegSlots*>(ws);
+  float* part = ws + p.part_off;
+  Share sh;
+  if (!share_init(p, sh)) return;
+  Range rg;
+  int c0, c1;
+  bool whole;
+  while (share_next(p, sh, rg, c0, c1, whole, slots)) {
+  const int b = sh.seg / a.H, h = sh.seg % a.H;
   const float w = a.w[h], r = a.r[h];
   const long long lens = rg.lens;
-  const int n = a.n;
+  __syncthreads();   // the previous piece is done with the shared arrays
   if (warp == 0) tree_nodes(a, b, nodes, lane);
   __syncthreads();
-  if (rg.nt > 0 && a.k) append_rows<float, float, D>(a, nodes, b, h, lens, c0, c1);
+  if (rg.any && a.k) append_rows<float, float, D>(a, nodes, b, h, lens, c0, c1);
   for (int i = warp; i < n; i += 4) {
     const float* q = reinterpret_cast<const float*>(a.q) + (long long)b * a.q_sb +
                      (long long)i * a.q_st + (long long)h * D;
@@ -52,7 +56,7 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(TreeParams p, float*
   float acc[PQ];
 #pragma unroll
   for (int x = 0; x < PQ; ++x) acc[x] = 0.f;
-  const int k0 = c0 * (kTile / kKeys), k1 = rg.nt > 0 ? (c1 + 1) * (kTile / kKeys) - 1 : k0 - 1;
+  const int k0 = c0 * (kTile / kKeys), k1 = rg.any ? (c1 + 1) * (kTile / kKeys) - 1 : k0 - 1;
   for (int tile = k0; tile <= k1; ++tile) {
     __syncthreads();
     if (tid < kKeys) {
@@ -125,21 +129,22 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(TreeParams p, float*
     float x[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) x[e] = lane + 32 * e < D ? qs[i * D + lane + 32 * e] : 0.f;
-    if (a.num_splits > 1) {
-      float* dst = part + (((size_t)bh * a.num_splits + split) * n + i) * D;
+    if (!whole) {
+      float* dst = part + ((size_t)(blockIdx.x + sh.seg) * n + i) * D;
 #pragma unroll
       for (int e = 0; e < PER; ++e)
         if (lane + 32 * e < D) dst[lane + 32 * e] = x[e];
     } else {
-      store_row<float, D>(a, b, i, h, lane, x, rg.nt > 0 && nodes.line[i] != 0);
+      store_row<float, D>(a, b, i, h, lane, x, rg.any && nodes.line[i] != 0);
     }
+  }
   }
 }
 
-// Sum the splits of a (sequence, head, node) in order, TanhNorm, store; a warp
-// per row.  The sum of an absent node is zero (nothing was seen).
+// Sum a segment's partials in the order of the list, TanhNorm, store; a warp per
+// (segment, node).  The sum of an absent node is zero (nothing was seen).
 template <typename TA, int D>
-__global__ void __launch_bounds__(128) tree_finish_kernel(TreeParams p, const float* __restrict__ part) {
+__global__ void __launch_bounds__(128) tree_finish_kernel(TreeParams p, const float* __restrict__ ws) {
   pdl_wait();
   pdl_trigger();
   constexpr int PER = D < 32 ? 1 : D / 32;
@@ -147,20 +152,19 @@ __global__ void __launch_bounds__(128) tree_finish_kernel(TreeParams p, const fl
   const int lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= (long long)a.B * a.H * a.n) return;
-  const int i = (int)(row % a.n);
-  const long long bh = row / a.n;
-  const int b = (int)(bh / a.H), h = (int)(bh % a.H);
-  const Range rg = tree_range(p, b, h);
+  const int i = (int)(row % a.n), seg = (int)(row / a.n);
+  const SegSlots q = reinterpret_cast<const SegSlots*>(ws)[seg];
+  if (q.last < q.first) return;   // written by the CTA that owned the segment
   float x[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) x[e] = 0.f;
-  const float* src = part + ((size_t)bh * a.num_splits * a.n + i) * D;
+  const float* src = ws + p.part_off + ((size_t)seg * a.n + i) * D;
 #pragma unroll 4
-  for (int s = 0; s < rg.used; ++s)
+  for (int c = q.first; c <= q.last; ++c)
 #pragma unroll
     for (int e = 0; e < PER; ++e)
-      if (lane + 32 * e < D) x[e] += src[(size_t)s * a.n * D + lane + 32 * e];
-  store_row<TA, D>(a, b, i, h, lane, x, true);
+      if (lane + 32 * e < D) x[e] += src[(size_t)c * a.n * D + lane + 32 * e];
+  store_row<TA, D>(a, seg / a.H, i, seg % a.H, lane, x, true);
 }
 
 template <int D>
@@ -168,8 +172,7 @@ void launch_f32(const TreeParams& p, float* part, cudaStream_t s) {
   const size_t smem = ((size_t)p.a.n * D + 2 * kKeys * (D + 4) + (size_t)p.a.n * 33) * 4;
   constexpr int kMost = (kMaxN * D + 2 * kKeys * (D + 4) + kMaxN * 33) * 4;
   if (ensure_smem_optin((const void*)tree_f32_kernel<D>, kMost) != cudaSuccess) return;
-  launch_pdl(tree_f32_kernel<D>, dim3(p.a.num_splits, p.a.B * p.a.H), dim3(kThreads), smem, s, p,
-             part);
+  launch_pdl(tree_f32_kernel<D>, tree_grid(p), dim3(kThreads), smem, s, p, part);
 }
 template <typename TA, int D>
 void launch_finish(const TreeParams& p, const float* part, cudaStream_t s) {

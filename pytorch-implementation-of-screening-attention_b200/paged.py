@@ -160,16 +160,16 @@ def paged_read(positions, n: int, k_pages, v_pages, block_table, k_scales=None, 
     return k, v
 
 
-def _tree_splits(bh: int, keys: int) -> int:
-    """Runs the key axis of one (sequence, head) is cut into, 64-key tiles."""
-    tiles = keys // 64 + 2
-    if tiles <= 8:
+def _tree_ctas(bh: int, keys: int) -> int:
+    """CTAs that the 64-key tiles of a call are shared out over; 1: one for each
+    of the bh (sequence, head) pairs, and no second launch."""
+    if keys // 64 + 2 <= 8 or bh > 2048:
         return 1
-    return max(1, min((tiles + 3) // 4, -(-148 * 6 // max(1, bh))))
+    return 148 * 3
 
 
 def _tree(fn, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_scales, v_scales,
-          max_window, num_splits, eps):
+          max_window, num_ctas, eps):
     desc, code, H, D = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
     dev = k_pages.device
     if q.dim() != 4:
@@ -191,9 +191,9 @@ def _tree(fn, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_sca
         return y
     table = block_table.shape[1] * k_pages.shape[2]
     keys = table if not max_window or max_window <= 0 else min(int(-(-max_window // 1)), table)
-    splits = _tree_splits(B * H, keys + n) if num_splits is None else int(num_splits)
+    ctas = _tree_ctas(B * H, keys + n) if num_ctas is None else int(num_ctas)
     a = _lib.TreeArgs(dtype=_lib._dtype_code(q), cache_dtype=code, B=B, H=H, D=D, n=n,
-                      num_splits=splits, max_window=keys, eps=float(eps),
+                      num_ctas=ctas, eps=float(eps),
                       q=q.data_ptr(), q_sb=q.stride(0), q_st=q.stride(1), lens=lens.data_ptr(),
                       r=r.data_ptr(), w=w.data_ptr(), cache=desc, k_scales=_lib._ptr(k_scales),
                       v_scales=_lib._ptr(v_scales), y=y.data_ptr())
@@ -206,7 +206,7 @@ def _tree(fn, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_sca
     if parents is not None:
         a.parents, a.parents_sb = parents.data_ptr(), parents.stride(0)
     lib = _lib.load()
-    if splits > 1:
+    if ctas > 1:
         need = lib.screen_tree_workspace_size(ctypes.byref(a))
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
@@ -215,10 +215,10 @@ def _tree(fn, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_sca
 
 
 def paged_decode(q, seq_lens, r, w, k_pages, v_pages, block_table, k_scales=None, v_scales=None,
-                 max_window=None, num_splits: int | None = None, eps: float = 1e-8):
+                 max_window=None, num_ctas: int | None = None, eps: float = 1e-8):
     """y (B, H, D) of raw q (B, H, D), the newest cached token of each sequence
     (position seq_lens[b] - 1, int32), over the window's cached keys.
-    `max_window` (the largest w) only sets how the key axis is shared out."""
+    `max_window` (the largest w) and num_ctas only set how the work is shared out."""
     if q.dim() != 3:
         raise ValueError("q must be (B, H, D)")
     if k_pages.dtype != torch.int8:
@@ -232,19 +232,21 @@ def paged_decode(q, seq_lens, r, w, k_pages, v_pages, block_table, k_scales=None
         _same_device(dev, q)
         seq_lens = _per_seq(seq_lens, B, dev, "seq_lens")
         r, w = _head_params(r, w, H, dev)
-        if num_splits is None:
-            table = block_table.shape[1] * k_pages.shape[2]
-            keys = table if not max_window or max_window <= 0 else min(int(-(-max_window // 1)), table)
-            num_splits = _tree_splits(B * H, keys)
+        table = block_table.shape[1] * k_pages.shape[2]
+        keys = table if not max_window or max_window <= 0 else min(int(-(-max_window // 1)), table)
+        if num_ctas is None:
+            num_ctas = _tree_ctas(B * H, keys)
+        # splits of every (sequence, head), at least a page each
+        num_splits = max(1, min(-(-num_ctas // max(1, B * H)), -(-keys // k_pages.shape[2])))
         with torch.cuda.device(dev):
             return _lib.screen_decode(q.detach(), seq_lens, r, w, k_pages, v_pages, block_table,
                                       eps, num_splits)[0]
     return _tree("screen_paged_decode_i8", q.unsqueeze(1), None, None, seq_lens, None, r, w, k_pages,
-                 v_pages, block_table, k_scales, v_scales, max_window, num_splits, eps).squeeze(1)
+                 v_pages, block_table, k_scales, v_scales, max_window, num_ctas, eps).squeeze(1)
 
 
 def paged_tree_decode(q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_scales=None,
-                      v_scales=None, max_window=None, num_splits: int | None = None,
+                      v_scales=None, max_window=None, num_ctas: int | None = None,
                       eps: float = 1e-8):
     """y (B, n, H, D) of a tree of n <= 64 drafted tokens per sequence, from raw
     q, k, v (B, n, H, D).
@@ -258,9 +260,10 @@ def paged_tree_decode(q, k, v, lens, parents, r, w, k_pages, v_pages, block_tabl
     depth: it sees the cached tokens of its window, its ancestors and itself.
     Every path of the tree gives what decoding its tokens one by one gives.  A
     ring table must hold ceil(max w) - 1 + n rows per sequence; nodes whose row
-    falls outside the table are not seen.  `max_window` as in paged_decode."""
+    falls outside the table are not seen.  `max_window` and num_ctas as in
+    paged_decode."""
     return _tree("screen_tree_decode", q, k, v, lens, parents, r, w, k_pages, v_pages, block_table,
-                 k_scales, v_scales, max_window, num_splits, eps)
+                 k_scales, v_scales, max_window, num_ctas, eps)
 
 
 def paged_commit(lens, path, counts, k_pages, v_pages, block_table, k_scales=None,

@@ -130,15 +130,15 @@ def bound(y, sums, r, dtype, i8):
 @pytest.mark.parametrize("B,H,D,ps,T,w", [(1, 1, 64, 64, 1, 2.0), (3, 2, 64, 64, 300, 130.5),
                                           (2, 3, 16, 8, 77, 500.0), (2, 2, 32, 24, 129, 64.0),
                                           (2, 2, 128, 100, 333, 1000.0), (1, 2, 64, 16, 1500, 1500.0)])
-@pytest.mark.parametrize("splits", [None, 1, 5])
-def test_decode(ms, dtype, B, H, D, ps, T, w, splits):
+@pytest.mark.parametrize("ctas", [None, 1, 5])
+def test_decode(ms, dtype, B, H, D, ps, T, w, ctas):
     (kp, vp, table, ks, vs), k, g = _filled(ms, B, H, D, ps, T, dtype, T + D)
     lens = torch.tensor([max(1, T - 11 * b) for b in range(B)], dtype=torch.int32)
     q = (k[:, -1] + 0.6 * torch.randn(B, H, D, generator=g)).to(dtype)
     r = torch.linspace(1.02, 1.9, H)
     ww = torch.linspace(w, max(1.5, w / 7), H)
     y = ms.paged_decode(q.to(DEV), lens.to(DEV), r.to(DEV), ww.to(DEV), kp, vp, table, ks, vs,
-                        max_window=w, num_splits=splits)
+                        max_window=w, num_ctas=ctas)
     cache = (kp.cpu(), vp.cpu(), ks.cpu(), vs.cpu(), table.cpu())
     for b in range(B):
         t = int(lens[b])

@@ -46,19 +46,19 @@ def test_append_and_read_codes(ms):
 
 def test_tree_codes(ms):
     L = ms._lib
-    ok = dict(dtype=L.BF16, cache_dtype=L.BF16, B=1, H=1, D=64, n=2, num_splits=1, eps=1e-8, q=16, q_sb=64, q_st=64,
+    ok = dict(dtype=L.BF16, cache_dtype=L.BF16, B=1, H=1, D=64, n=2, num_ctas=1, eps=1e-8, q=16, q_sb=64, q_st=64,
               k=16, k_sb=64, k_st=64, v=32, v_sb=64, v_st=64, lens=64, r=64, w=64, y=128)
     for bad, code in ((dict(dtype=2), -3), (dict(cache_dtype=L.F32), -3), (dict(D=20), -2), (dict(n=65), -1),
-                      (dict(n=-1), -1), (dict(num_splits=0), -1), (dict(lens=None), -1), (dict(v=None), -1),
+                      (dict(n=-1), -1), (dict(num_ctas=0), -1), (dict(lens=None), -1), (dict(v=None), -1),
                       (dict(cache_dtype=L.I8), -1), (dict(q=24), -4), (dict(k_st=2), -4), (dict(y=136), -4),
-                      (dict(num_splits=2), -5), (dict(num_splits=2, workspace=256, workspace_bytes=16), -5),
-                      (dict(B=70000), -9), (dict(n=0), 0), (dict(B=0), 0)):
+                      (dict(num_ctas=2), -5), (dict(num_ctas=2, workspace=256, workspace_bytes=16), -5),
+                      (dict(num_ctas=70000), -1), (dict(n=0), 0), (dict(B=0), 0)):
         assert call(L, "screen_tree_decode", L.TreeArgs(**{**ok, "cache": desc(L), **bad})) == code, bad
     one = {**ok, "cache": desc(L), "n": 1, "k": None, "v": None, "cache_dtype": L.I8, "k_scales": 64, "v_scales": 64}
     for bad, code in ((dict(cache_dtype=L.BF16), -3), (dict(n=2), -1), (dict(k=16, v=16), -1), (dict(parents=64), -1),
                       (dict(B=0), 0)):
         assert call(L, "screen_paged_decode_i8", L.TreeArgs(**{**one, **bad})) == code, bad
-    a = L.TreeArgs(**{**ok, "cache": desc(L), "num_splits": 3})
+    a = L.TreeArgs(**{**ok, "cache": desc(L), "num_ctas": 3})
     assert L.load().screen_tree_workspace_size(ctypes.byref(a)) >= 3 * 2 * 64 * 4
 
 

@@ -34,7 +34,7 @@ def test_refusals(ms):
                dict(k=q.float()), dict(q=q.half(), k=q.half(), v=q.half(), kp=k8, vp=k8, ks=sc, vs=sc)):
         with pytest.raises(TypeError):
             tree(**kw)
-    for kw in (dict(q=q.cpu()), dict(lens=lens.cpu()), dict(k=q.cpu()), dict(table=table.cpu()), dict(num_splits=0)):
+    for kw in (dict(q=q.cpu()), dict(lens=lens.cpu()), dict(k=q.cpu()), dict(table=table.cpu()), dict(num_ctas=0)):
         with pytest.raises(RuntimeError):
             tree(**kw)
     with pytest.raises(TypeError):

@@ -95,16 +95,16 @@ def test_tree(ms, B, H, D, ps, T, n, dtype, q8, kind):
 
 @pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True),
                                       (torch.float32, False), (torch.float32, True)])
-@pytest.mark.parametrize("splits", [1, 2, 7, 40])
-def test_splits_agree(ms, dtype, q8, splits):
-    """Any number of splits, and any hint of the window, gives the same rows to
+@pytest.mark.parametrize("ctas", [1, 2, 7, 40])
+def test_ctas_agree(ms, dtype, q8, ctas):
+    """Any number of CTAs, and any hint of the window, gives the same rows to
     the order of the sums; twice the same call gives the same bits."""
     c = make(ms, 2, 2, 64, 16, 500, 9, dtype, q8, 5)
     lens = torch.tensor([500, 444], dtype=torch.int32)
     parents = tree_parents(2, 9, "random", c["g"])
     r, w = torch.tensor([1.1, 1.4]), torch.tensor([600.0, 90.0])
-    y = check(ms, c, lens, parents, r, w, dtype, q8, num_splits=splits, max_window=3)
-    z = check(ms, c, lens, parents, r, w, dtype, q8, num_splits=splits, max_window=3)
+    y = check(ms, c, lens, parents, r, w, dtype, q8, num_ctas=ctas, max_window=3)
+    z = check(ms, c, lens, parents, r, w, dtype, q8, num_ctas=ctas, max_window=3)
     assert torch.equal(y, z)
 
 
@@ -257,7 +257,7 @@ def test_captured_and_on_two_streams(ms, q8):
 
     def run(c):
         return ms.paged_tree_decode(c["dq"], c["dk"], c["dv"], lens, None, r, w, c["kp"], c["vp"], c["table"], c["ks"],
-                                    c["vs"], num_splits=4)
+                                    c["vs"], num_ctas=4)
 
     for c in cs:
         c["dq"], c["dk"], c["dv"] = (c[x].to(DEV) for x in "qkv")
