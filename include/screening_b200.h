@@ -364,6 +364,7 @@ typedef struct screen_verify_args {
   void* workspace; size_t workspace_bytes;
 } screen_verify_args;
 
+/* Bytes of device workspace screen_verify_drafts needs (0 for many rows). */
 SCREEN_API size_t screen_verify_workspace_size(const screen_verify_args* a);
 
 /* Speculative sampling.  Logits row 0 follows the newest token, row 1 + i

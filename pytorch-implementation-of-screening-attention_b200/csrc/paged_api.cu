@@ -134,7 +134,7 @@ int screen_paged_commit(const screen_commit_args* a, screen_stream_t stream) {
 }
 
 size_t screen_verify_workspace_size(const screen_verify_args* a) {
-  if (!a || a->B < 0 || a->n < 0) return 0;
+  if (!a || a->B <= 0 || a->n < 0 || a->V < 1) return 0;
   return round_up(verify_workspace(*a));
 }
 
@@ -150,8 +150,8 @@ int screen_verify_drafts(const screen_verify_args* a, screen_stream_t stream) {
     return SCREEN_ERR_INVALID_ARG;
   if (a->B > (1 << 24)) return SCREEN_ERR_UNSUPPORTED;
   const size_t need = screen_verify_workspace_size(a);
-  if (!a->workspace || a->workspace_bytes < need) return SCREEN_ERR_WORKSPACE;
-  if (!al16(a->workspace)) return SCREEN_ERR_ALIGNMENT;
+  if (need && (!a->workspace || a->workspace_bytes < need)) return SCREEN_ERR_WORKSPACE;
+  if (need && !al16(a->workspace)) return SCREEN_ERR_ALIGNMENT;
   verify(*a, (cudaStream_t)stream);
   return check_launch();
 }

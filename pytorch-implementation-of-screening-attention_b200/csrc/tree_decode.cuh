@@ -260,8 +260,12 @@ __device__ __forceinline__ void store_row(const screen_tree_args& a, int b, int 
     if (lane + 32 * e < D) y[lane + 32 * e] = from_f<TA>(present ? o[e] * g : 0.f);
 }
 
-inline dim3 tree_grid(const TreeParams& p) {
-  return dim3(p.a.num_ctas == 1 ? p.a.B * p.a.H : p.a.num_ctas);
+// One CTA per segment, or at most as many as are resident at once: a run for
+// each, all of one length.
+constexpr int kSMs = 148;
+inline dim3 tree_grid(const TreeParams& p, int per_sm) {
+  if (p.a.num_ctas == 1) return dim3(p.a.B * p.a.H);
+  return dim3(p.a.num_ctas < kSMs * per_sm ? p.a.num_ctas : kSMs * per_sm);
 }
 
 }  // namespace tree

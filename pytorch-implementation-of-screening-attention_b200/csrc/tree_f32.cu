@@ -172,7 +172,7 @@ void launch_f32(const TreeParams& p, float* part, cudaStream_t s) {
   const size_t smem = ((size_t)p.a.n * D + 2 * kKeys * (D + 4) + (size_t)p.a.n * 33) * 4;
   constexpr int kMost = (kMaxN * D + 2 * kKeys * (D + 4) + kMaxN * 33) * 4;
   if (ensure_smem_optin((const void*)tree_f32_kernel<D>, kMost) != cudaSuccess) return;
-  launch_pdl(tree_f32_kernel<D>, tree_grid(p), dim3(kThreads), smem, s, p, part);
+  launch_pdl(tree_f32_kernel<D>, tree_grid(p, 3), dim3(kThreads), smem, s, p, part);
 }
 template <typename TA, int D>
 void launch_finish(const TreeParams& p, const float* part, cudaStream_t s) {

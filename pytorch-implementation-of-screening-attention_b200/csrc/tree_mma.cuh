@@ -7,9 +7,17 @@
 namespace screen {
 namespace tree {
 
+// Not volatile: a product depends on its operands only, and the compiler may
+// interleave independent chains.
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_b16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -65,7 +73,7 @@ struct Cfg {
   static constexpr int SMEM = RING_B > RED_B ? RING_B : RED_B;
   // CTAs per SM the registers are cut to: what a thread holds of O and q decides
   static constexpr int HELD = QW_ * (D_ / 2 + D_ / 4 * (QHL ? 2 : 1));
-  static constexpr int MINB = HELD <= 32 ? 4 : HELD <= 64 ? 3 : 2;
+    static constexpr int MINB = HELD <= 32 ? 4 : HELD <= 64 ? 3 : 2;
 };
 
 // Byte offset of 16-byte chunk c of key row r inside a tile.  The XOR makes the
@@ -450,48 +458,70 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
           const bool edge = cpos[KT] != 0;
           slot = slot + 1 == S ? 0 : slot + 1;
           fill = fill + 1 == S ? 0 : fill + 1;
-#pragma unroll 1
+#pragma unroll
           for (int kg = 0; kg < KT / 16; ++kg) {
             float2 s[QW][2][RH];                       // keys 2t, 2t + 1 of an 8-key tile
             float tmax = 0.f;
+            {
+              uint32_t kb[2][C::KS][2];
+              float c[2][QW][4], d[C::QHL ? 2 : 1][QW][4];
+              float2 ks[2];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-              const int base = kg * 16 + nt * 8;
-              uint32_t kb[C::KS][2];
-              load_k<C>(kt, base + key_of<C>(g), t, kb);
-              float2 ks = both(1.f);
-              if constexpr (C::I8) ks = *reinterpret_cast<const float2*>(cs + 2 * KT + base + 2 * t);
+              for (int nt = 0; nt < 2; ++nt) {
+                const int base = kg * 16 + nt * 8;
+                load_k<C>(kt, base + key_of<C>(g), t, kb[nt]);
+                ks[nt] = both(1.f);
+                if constexpr (C::I8)
+                  ks[nt] = *reinterpret_cast<const float2*>(cs + 2 * KT + base + 2 * t);
 #pragma unroll
-              for (int m = 0; m < QW; ++m) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (C::QHL) {
-                  // the small products first, two short chains: the tensor
-                  // core's sums truncate
-                  float d[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int m = 0; m < QW; ++m)
 #pragma unroll
-                  for (int x2 = 0; x2 < C::KS; ++x2)
-                    mma_f16(x2 & 1 ? d : c, ql[m][x2], kb[x2][0], kb[x2][1]);
-#pragma unroll
-                  for (int x2 = 0; x2 < C::KS; ++x2)
-                    mma_f16(x2 & 1 ? d : c, qa[m][x2], kb[x2][0], kb[x2][1]);
-#pragma unroll
-                  for (int f = 0; f < 4; ++f) c[f] += d[f];
-                } else {
-#pragma unroll
-                  for (int x2 = 0; x2 < C::KS; ++x2) {
-                    if constexpr (C::I8) mma_f16(c, qa[m][x2], kb[x2][0], kb[x2][1]);
-                    else mma_bf16(c, qa[m][x2], kb[x2][0], kb[x2][1]);
+                  for (int f = 0; f < 4; ++f) {
+                    c[nt][m][f] = 0.f;
+                    if constexpr (C::QHL) d[nt][m][f] = 0.f;
                   }
-                }
-#pragma unroll
-                for (int e = 0; e < RH; ++e) {
-                  float2 v = make_float2(c[2 * e], c[2 * e + 1]);
-                  if constexpr (C::I8) v = mul2(v, ks);
-                  v = fma2(v, both(rq[m][e]), one_r);
-                  // NaN (an unseen row, a non-finite key) counts as 0
-                  s[m][nt][e] = make_float2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f));
-                }
               }
+              // k step outermost: 2 QW independent chains of products
+              if constexpr (C::QHL) {
+                // the small products first, and two chains: the tensor core's
+                // sums truncate
+#pragma unroll
+                for (int x2 = 0; x2 < C::KS; ++x2)
+#pragma unroll
+                  for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int m = 0; m < QW; ++m)
+                      mma_f16(x2 & 1 ? d[nt][m] : c[nt][m], ql[m][x2], kb[nt][x2][0], kb[nt][x2][1]);
+              }
+#pragma unroll
+              for (int x2 = 0; x2 < C::KS; ++x2)
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                  for (int m = 0; m < QW; ++m) {
+                    if constexpr (C::QHL)
+                      mma_f16(x2 & 1 ? d[nt][m] : c[nt][m], qa[m][x2], kb[nt][x2][0], kb[nt][x2][1]);
+                    else if constexpr (C::I8)
+                      mma_f16(c[nt][m], qa[m][x2], kb[nt][x2][0], kb[nt][x2][1]);
+                    else
+                      mma_b16(c[nt][m], qa[m][x2], kb[nt][x2][0], kb[nt][x2][1]);
+                  }
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int m = 0; m < QW; ++m)
+#pragma unroll
+                  for (int e = 0; e < RH; ++e) {
+                    float2 v = make_float2(c[nt][m][2 * e], c[nt][m][2 * e + 1]);
+                    if constexpr (C::QHL) {
+                      v.x += d[nt][m][2 * e];
+                      v.y += d[nt][m][2 * e + 1];
+                    }
+                    if constexpr (C::I8) v = mul2(v, ks[nt]);
+                    v = fma2(v, both(rq[m][e]), one_r);
+                    // NaN (an unseen row, a non-finite key) counts as 0
+                    s[m][nt][e] = make_float2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f));
+                  }
             }
             if (edge) {
 #pragma unroll
@@ -605,8 +635,8 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
                 } else if constexpr (C::I8) {
                   mma_f16(o[m][j], pa, vb[j][0], vb[j][1]);
                 } else {
-                  mma_bf16(o[m][j], pa, vb[j][0], vb[j][1]);
-                  mma_bf16(o[m][j], pl, vb[j][0], vb[j][1]);
+                  mma_b16(o[m][j], pa, vb[j][0], vb[j][1]);
+                  mma_b16(o[m][j], pl, vb[j][0], vb[j][1]);
                 }
               }
             }
@@ -665,14 +695,15 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
 template <class C>
 void launch_tree(const TreeParams& p, float* ws, cudaStream_t s) {
   if (ensure_smem_optin((const void*)tree_mma_kernel<C>, C::SMEM) != cudaSuccess) return;
-  launch_pdl(tree_mma_kernel<C>, tree_grid(p), dim3(kThreads), (size_t)C::SMEM, s, p, ws);
+  launch_pdl(tree_mma_kernel<C>, tree_grid(p, C::MINB), dim3(kThreads),
+             (size_t)C::SMEM, s, p, ws);
 }
 // Query tiles per warp: two where the registers allow it (D <= 64) and there
 // are more than 16 queries, so that a K / V fragment feeds two products; up to
 // 8 queries the lower half of a tile is not computed on.
 template <typename E, typename TA, int D>
 void launch_tree_d(const TreeParams& p, float* ws, cudaStream_t s) {
-  constexpr int Q2 = D <= 64 ? 2 : 1;
+    constexpr int Q2 = D <= 64 ? 2 : 1;
   if (p.a.n <= 8) launch_tree<Cfg<E, TA, D, 1, 1, 1>>(p, ws, s);
   else if (p.a.n <= 16) launch_tree<Cfg<E, TA, D, 1, 1, 2>>(p, ws, s);
   else if (p.a.n <= 32) launch_tree<Cfg<E, TA, D, Q2, 2 / Q2, 2>>(p, ws, s);

@@ -161,11 +161,12 @@ def paged_read(positions, n: int, k_pages, v_pages, block_table, k_scales=None, 
 
 
 def _tree_ctas(bh: int, keys: int) -> int:
-    """CTAs that the 64-key tiles of a call are shared out over; 1: one for each
-    of the bh (sequence, head) pairs, and no second launch."""
+    """CTAs that the 64-key tiles of a call are shared out over, at most (the
+    library takes as many as run at once); 1: one for each of the bh (sequence,
+    head) pairs, and no second launch."""
     if keys // 64 + 2 <= 8 or bh > 2048:
         return 1
-    return 148 * 3
+    return 148 * 4
 
 
 def _tree(fn, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_scales, v_scales,
@@ -373,10 +374,11 @@ def verify_drafts(logits, tokens, parents, uniforms, draft_logits=None, temperat
     counts = torch.empty((B,), dtype=torch.int32, device=dev)
     if B == 0:
         return out, path, counts
+    a.out_tokens, a.path, a.counts = out.data_ptr(), path.data_ptr(), counts.data_ptr()
     lib = _lib.load()
     need = lib.screen_verify_workspace_size(ctypes.byref(a))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    a.out_tokens, a.path, a.counts = out.data_ptr(), path.data_ptr(), counts.data_ptr()
-    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
     _run(lib.screen_verify_drafts, a, dev)
     return out, path, counts

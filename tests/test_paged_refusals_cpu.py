@@ -26,7 +26,7 @@ def test_struct_sizes(ms):
     for f in ("screen_paged_append_i8", "screen_paged_read", "screen_tree_decode", "screen_paged_decode_i8",
               "screen_paged_commit", "screen_verify_drafts"):
         assert getattr(lib, f)(None, None) == -1
-    assert lib.screen_tree_workspace_size(None) == 0 and lib.screen_verify_workspace_size(None) == 0
+    assert lib.screen_tree_workspace_size(None) == 0
 
 
 def test_append_and_read_codes(ms):
@@ -74,7 +74,8 @@ def test_commit_and_verify_codes(ms):
     for bad, code in ((dict(dtype=2), -3), (dict(n=65), -1), (dict(n=-1), -1), (dict(V=0), -1),
                       (dict(temperature=-1.0), -1), (dict(temperature=float("nan")), -1),
                       (dict(temperature=float("inf")), -1), (dict(logits=None), -1), (dict(tokens=None), -1),
-                      (dict(path=None), -1), (dict(workspace=None), -5), (dict(workspace_bytes=1), -5), (dict(B=0), 0)):
+                      (dict(path=None), -1), (dict(workspace=None), -5), (dict(workspace_bytes=1), -5),
+                      (dict(workspace=264), -4), (dict(B=0), 0)):
         assert call(L, "screen_verify_drafts", L.VerifyArgs(**{**ok, **bad})) == code, bad
 
 
