@@ -12,7 +12,7 @@ prefix for every token (multiscreen/model.py:131-133).
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
@@ -21,83 +21,147 @@ from . import _lib
 _PAGE_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.int8: _lib.I8}
 MAX_NODES = _lib.TREE_MAX_NODES
 
+# A call's arguments are packed straight into the bytes of its C struct
+# (include/screening_b200.h; native alignment): building the ctypes mirror field by
+# field cost as much as the shortest of these kernels runs.  _entry() checks the
+# sizes against the mirrors.
+_CACHE = "3P4i"
+_LAYOUTS = {
+    "screen_kv_append": ("5if P2q P2q P" + _CACHE + "0q", _lib.KVAppendArgs),
+    "screen_paged_append_i8": ("5if P2q P2q P" + _CACHE + "2P0q", _lib.PagedAppendArgs),
+    "screen_paged_read": ("6i2P P" + _CACHE + "2P0q", _lib.PagedReadArgs),
+    "screen_tree_decode": ("7if P2q P2q P2q 2Pq 2P" + _CACHE + "2P 2PN0q", _lib.TreeArgs),
+    "screen_paged_commit": ("6i 2PqP" + _CACHE + "2Pq0q", _lib.CommitArgs),
+    "screen_verify_drafts": ("4ifi P P2q P2q Pq Pq Pq 3P PN0q", _lib.VerifyArgs),
+}
+_LAYOUTS["screen_paged_decode_i8"] = _LAYOUTS["screen_tree_decode"]
+_entries = {}
 
-def _same_device(dev, *ts):
-    for t in ts:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"expected every tensor on {dev}, got one on {t.device}")
+
+def _entry(name):
+    """(pack, call) of a C entry point."""
+    e = _entries.get(name)
+    if e is None:
+        import ctypes
+        lib = _lib.load()
+        fmt, mirror = _LAYOUTS[name]
+        st = struct.Struct(fmt.replace(" ", ""))
+        if st.size != ctypes.sizeof(mirror):
+            raise RuntimeError(f"{name}: packed arguments differ from {mirror.__name__}")
+        proto = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)
+        e = _entries[name] = (st.pack, proto(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value))
+    return e
 
 
-def _run(fn, args, dev):
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
-        _lib._check(fn(ctypes.byref(args), stream))
+def _size_query(name):
+    """A workspace size query on packed arguments."""
+    q = _entries.get(name)
+    if q is None:
+        import ctypes
+        proto = ctypes.CFUNCTYPE(ctypes.c_size_t, ctypes.c_char_p)
+        q = _entries[name] = proto(ctypes.cast(getattr(_lib.load(), name), ctypes.c_void_p).value)
+    return q
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _run(call, args, index):
+    """The call on the current stream of CUDA device `index`."""
+    if torch.cuda.current_device() == index:
+        status = call(args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            _lib._check(fn(ctypes.byref(args), stream))
+        with torch.cuda.device(index):
+            status = call(args, _raw_stream(index))
+    if status:
+        _lib._check(status)
+
+
+def _same_device(index, *ts):
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            _lib._require_cuda(t)
+            raise RuntimeError(f"expected every tensor on cuda:{index}, got one on {t.device}")
 
 
 def _pages(k_pages, v_pages, block_table, k_scales, v_scales, ndim=4):
-    """Checks a cache; returns (descriptor, dtype code, H, D, block table)."""
-    _lib._require_cuda(k_pages, v_pages, block_table, k_scales, v_scales)
-    _same_device(k_pages.device, v_pages, block_table, k_scales, v_scales)
-    code = _PAGE_DTYPES.get(k_pages.dtype)
-    if code is None or v_pages.dtype != k_pages.dtype:
+    """Checks a cache; returns (device index, dtype code, shape, its packed
+    arguments (pages, table, sizes), the scales' pointers)."""
+    index = k_pages.get_device()
+    if index < 0:
+        _lib._require_cuda(k_pages)
+    _same_device(index, v_pages, block_table, k_scales, v_scales)
+    dtype, shape = k_pages.dtype, k_pages.shape
+    code = _PAGE_DTYPES.get(dtype)
+    if code is None or v_pages.dtype is not dtype:
         raise TypeError(f"pages are float32, bfloat16 or int8, both alike; got {k_pages.dtype} "
                         f"and {v_pages.dtype}")
-    if k_pages.dim() != ndim or v_pages.shape != k_pages.shape:
+    if len(shape) != ndim or v_pages.shape != shape:
         raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)}: "
                          "expected two of [num_pages, H, page_size, D]")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("pages must be contiguous")
     if (code == _lib.I8) != (k_scales is not None) or (k_scales is None) != (v_scales is None):
         raise ValueError("int8 pages come with k_scales and v_scales, other pages with neither")
-    for s in (k_scales, v_scales):
-        if s is not None and (s.dtype != torch.float32 or s.shape != k_pages.shape[:-1]
-                              or not s.is_contiguous()):
-            raise ValueError("scales must be contiguous float32 of the pages' shape without D")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous():
+    scales = (0, 0)
+    if k_scales is not None:
+        for s in (k_scales, v_scales):
+            if s.dtype is not torch.float32 or s.shape != shape[:-1] or not s.is_contiguous():
+                raise ValueError("scales must be contiguous float32 of the pages' shape without D")
+        scales = (k_scales.data_ptr(), v_scales.data_ptr())
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous():
         raise ValueError("block_table must be a contiguous int32 [B, max_blocks]")
-    P, H, ps, D = k_pages.shape[-4:]
-    desc = _lib.KVCacheDesc(k_pages=k_pages.data_ptr(), v_pages=v_pages.data_ptr(),
-                            block_table=block_table.data_ptr(), num_pages=P, page_size=ps,
-                            max_blocks=block_table.shape[1])
-    return desc, code, H, D
+    P, H, ps, D = shape[-4:]
+    return index, code, shape, (k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), P, ps,
+                                block_table.shape[1], 0), scales
 
 
-def _per_seq(t, B, dev, name):
-    _lib._require_cuda(t)
-    _same_device(dev, t)
-    if t.dtype != torch.int32 or t.shape != (B,):
+def _per_seq(t, B, index, name):
+    if t.get_device() != index:
+        _same_device(index, t)
+    if t.dtype is not torch.int32 or t.shape != (B,):
         raise ValueError(f"{name} must be int32 of shape ({B},), got {t.dtype} {tuple(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _node_ints(t, B, n, dev, name):
+def _node_ints(t, B, n, index, name):
     """An int32 (B, n) tensor with unit stride over n, or None."""
     if t is None:
         return None
-    _lib._require_cuda(t)
-    _same_device(dev, t)
-    if t.dtype != torch.int32 or t.shape != (B, n):
+    if t.get_device() != index:
+        _same_device(index, t)
+    if t.dtype is not torch.int32 or t.shape != (B, n):
         raise ValueError(f"{name} must be int32 of shape ({B}, {n}), got {t.dtype} {tuple(t.shape)}")
     return t if n == 0 or t.stride(1) == 1 else t.contiguous()
 
 
-def _head_params(r, w, H, dev):
-    _lib._require_cuda(r, w)
-    _same_device(dev, r, w)
+def _head_params(r, w, H, index):
+    _same_device(index, r, w)
     if r.shape != (H,) or w.shape != (H,):
         raise ValueError(f"r and w must have shape ({H},)")
-    return r.detach().float().contiguous(), w.detach().float().contiguous()
+    if r.dtype is not torch.float32 or not r.is_contiguous():
+        r = r.detach().float().contiguous()
+    if w.dtype is not torch.float32 or not w.is_contiguous():
+        w = w.detach().float().contiguous()
+    return r, w
 
 
-def _rows(x, B, n, H, D, dev, name):
-    _lib._require_cuda(x)
-    _same_device(dev, x)
-    if x.shape != (B, n, H, D):
-        raise ValueError(f"{name} must have shape {(B, n, H, D)}, got {tuple(x.shape)}")
-    return _lib._bthd(x.detach())
+def _rows(x, shape, index, name):
+    """(tensor to keep, pointer, batch stride, row stride) of raw rows the
+    kernels read in place where their layout allows it."""
+    if x.get_device() != index:
+        _same_device(index, x)
+    if x.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
+    sb, st, sh, sd = x.stride()
+    vec = 8 if x.dtype is torch.bfloat16 else 4
+    p = x.data_ptr()
+    if sd != 1 or sh != shape[3] or sb % vec or st % vec or p % 16:
+        x = x.detach().contiguous()
+        sb, st, _, _ = x.stride()
+        p = x.data_ptr()
+    return x, p, sb, st
 
 
 def _table_batch(block_table, B):
@@ -112,28 +176,25 @@ def paged_append(k, v, positions, k_pages, v_pages, block_table, k_scales=None, 
     1 / max(|m|, 127 eps / max|x|) per row, so that scale * m is a unit row; k, v
     are then float32 or bfloat16, otherwise of the pages' dtype.  Positions
     outside the block table are skipped."""
-    desc, code, H, D = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
-    dev = k_pages.device
-    if k.dim() != 4 or v.dtype != k.dtype:
+    index, code, shape, cache, scales = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
+    if k.dim() != 4 or v.dtype is not k.dtype:
         raise ValueError("k and v must be (B, n, H, D) of one dtype")
     B, n = k.shape[:2]
-    k, v = _rows(k, B, n, H, D, dev, "k"), _rows(v, B, n, H, D, dev, "v")
-    positions = _per_seq(positions, B, dev, "positions")
+    H, D = shape[1], shape[3]
+    k, kp, k_sb, k_st = _rows(k, (B, n, H, D), index, "k")
+    v, vp, v_sb, v_st = _rows(v, (B, n, H, D), index, "v")
+    positions = _per_seq(positions, B, index, "positions")
     _table_batch(block_table, B)
-    if code != _lib.I8:
-        if k.dtype != k_pages.dtype:
-            raise TypeError("cache dtype must match k/v")
-        a = _lib.KVAppendArgs(dtype=code, B=B, H=H, D=D, n_new=n, eps=float(eps),
-                              k=k.data_ptr(), k_sb=k.stride(0), k_st=k.stride(1),
-                              v=v.data_ptr(), v_sb=v.stride(0), v_st=v.stride(1),
-                              positions=positions.data_ptr(), cache=desc)
-        return _run(_lib.load().screen_kv_append, a, dev)
-    a = _lib.PagedAppendArgs(dtype=_lib._dtype_code(k), B=B, H=H, D=D, n_new=n, eps=float(eps),
-                             k=k.data_ptr(), k_sb=k.stride(0), k_st=k.stride(1),
-                             v=v.data_ptr(), v_sb=v.stride(0), v_st=v.stride(1),
-                             positions=positions.data_ptr(), cache=desc,
-                             k_scales=k_scales.data_ptr(), v_scales=v_scales.data_ptr())
-    return _run(_lib.load().screen_paged_append_i8, a, dev)
+    if code == _lib.I8:
+        pack, call = _entry("screen_paged_append_i8")
+        _run(call, pack(_lib._dtype_code(k), B, H, D, n, eps, kp, k_sb, k_st, vp, v_sb, v_st,
+                        positions.data_ptr(), *cache, *scales), index)
+        return
+    if k.dtype is not k_pages.dtype:
+        raise TypeError("cache dtype must match k/v")
+    pack, call = _entry("screen_kv_append")
+    _run(call, pack(code, B, H, D, n, eps, kp, k_sb, k_st, vp, v_sb, v_st, positions.data_ptr(),
+                    *cache), index)
 
 
 def paged_read(positions, n: int, k_pages, v_pages, block_table, k_scales=None, v_scales=None,
@@ -141,22 +202,20 @@ def paged_read(positions, n: int, k_pages, v_pages, block_table, k_scales=None, 
     """(k, v) (B, n, H, D): the values of the cached rows at positions[b] +
     (0 .. n-1), in `dtype` (float32 or bfloat16; default the pages' own, float32
     for int8).  Rows outside the block table are zero."""
-    desc, code, H, D = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
-    dev = k_pages.device
-    B = block_table.shape[0]
-    positions = _per_seq(positions, B, dev, "positions")
+    index, code, shape, cache, scales = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
+    B, H, D = block_table.shape[0], shape[1], shape[3]
+    positions = _per_seq(positions, B, index, "positions")
     if n < 0:
         raise ValueError("n must not be negative")
     if dtype is None:
         dtype = torch.float32 if code == _lib.I8 else k_pages.dtype
     if dtype not in _lib._DTYPES:
         raise TypeError(f"rows are read as float32 or bfloat16, got {dtype}")
-    k = torch.empty((B, n, H, D), dtype=dtype, device=dev)
+    k = torch.empty((B, n, H, D), dtype=dtype, device=k_pages.device)
     v = torch.empty_like(k)
-    a = _lib.PagedReadArgs(dtype=_lib._DTYPES[dtype], cache_dtype=code, B=B, H=H, D=D, n=int(n),
-                           k=k.data_ptr(), v=v.data_ptr(), positions=positions.data_ptr(),
-                           cache=desc, k_scales=_lib._ptr(k_scales), v_scales=_lib._ptr(v_scales))
-    _run(_lib.load().screen_paged_read, a, dev)
+    pack, call = _entry("screen_paged_read")
+    _run(call, pack(_lib._DTYPES[dtype], code, B, H, D, int(n), k.data_ptr(), v.data_ptr(),
+                    positions.data_ptr(), *cache, *scales), index)
     return k, v
 
 
@@ -169,49 +228,54 @@ def _tree_ctas(bh: int, keys: int) -> int:
     return 148 * 4
 
 
-def _tree(fn, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_scales, v_scales,
+def _keys_seen(max_window, block_table, page_size):
+    table = block_table.shape[1] * page_size
+    return table if not max_window or max_window <= 0 else min(int(-(-max_window // 1)), table)
+
+
+def _tree(name, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_scales, v_scales,
           max_window, num_ctas, eps):
-    desc, code, H, D = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
-    dev = k_pages.device
+    index, code, shape, cache, scales = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
     if q.dim() != 4:
         raise ValueError("q must be (B, n, H, D)")
     B, n = q.shape[:2]
-    q = _rows(q, B, n, H, D, dev, "q")
-    if code != _lib.I8 and q.dtype != k_pages.dtype:
+    H, D = shape[1], shape[3]
+    full = (B, n, H, D)
+    q, qp, q_sb, q_st = _rows(q, full, index, "q")
+    dtype = q.dtype
+    if code != _lib.I8 and dtype is not k_pages.dtype:
         raise TypeError(f"q is {q.dtype}, the cache {k_pages.dtype}")
     if n > MAX_NODES:
         raise ValueError(f"a tree has at most {MAX_NODES} nodes, got {n}")
     _table_batch(block_table, B)
-    lens = _per_seq(lens, B, dev, "lens")
-    parents = _node_ints(parents, B, n, dev, "parents")
-    r, w = _head_params(r, w, H, dev)
+    lens = _per_seq(lens, B, index, "lens")
+    parents = _node_ints(parents, B, n, index, "parents")
+    r, w = _head_params(r, w, H, index)
+    kp = k_sb = k_st = vp = v_sb = v_st = 0
     if (k is None) != (v is None):
         raise ValueError("k and v are given together")
-    y = torch.empty((B, n, H, D), dtype=q.dtype, device=dev)
-    if y.numel() == 0:
-        return y
-    table = block_table.shape[1] * k_pages.shape[2]
-    keys = table if not max_window or max_window <= 0 else min(int(-(-max_window // 1)), table)
-    ctas = _tree_ctas(B * H, keys + n) if num_ctas is None else int(num_ctas)
-    a = _lib.TreeArgs(dtype=_lib._dtype_code(q), cache_dtype=code, B=B, H=H, D=D, n=n,
-                      num_ctas=ctas, eps=float(eps),
-                      q=q.data_ptr(), q_sb=q.stride(0), q_st=q.stride(1), lens=lens.data_ptr(),
-                      r=r.data_ptr(), w=w.data_ptr(), cache=desc, k_scales=_lib._ptr(k_scales),
-                      v_scales=_lib._ptr(v_scales), y=y.data_ptr())
     if k is not None:
-        k, v = _rows(k, B, n, H, D, dev, "k"), _rows(v, B, n, H, D, dev, "v")
-        if k.dtype != q.dtype or v.dtype != q.dtype:
+        if k.dtype is not dtype or v.dtype is not dtype:
             raise TypeError("q, k, v must share a dtype")
-        a.k, a.k_sb, a.k_st = k.data_ptr(), k.stride(0), k.stride(1)
-        a.v, a.v_sb, a.v_st = v.data_ptr(), v.stride(0), v.stride(1)
-    if parents is not None:
-        a.parents, a.parents_sb = parents.data_ptr(), parents.stride(0)
-    lib = _lib.load()
-    if ctas > 1:
-        need = lib.screen_tree_workspace_size(ctypes.byref(a))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    _run(getattr(lib, fn), a, dev)
+        k, kp, k_sb, k_st = _rows(k, full, index, "k")
+        v, vp, v_sb, v_st = _rows(v, full, index, "v")
+    y = q.new_empty(full)
+    dcode = _lib._dtype_code(q)
+    if B * n * H == 0:
+        return y
+    if num_ctas is None:
+        num_ctas = _tree_ctas(B * H, _keys_seen(max_window, block_table, shape[2]) + n)
+    pack, call = _entry(name)
+    pp, p_sb = (0, 0) if parents is None else (parents.data_ptr(), parents.stride(0))
+    args = (dcode, code, B, H, D, n, int(num_ctas), eps, qp, q_sb, q_st, kp, k_sb, k_st, vp, v_sb,
+            v_st, lens.data_ptr(), pp, p_sb, r.data_ptr(), w.data_ptr(), *cache, *scales,
+            y.data_ptr())
+    if num_ctas > 1:
+        need = _size_query("screen_tree_workspace_size")(pack(*args, 0, 0))
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _run(call, pack(*args, ws.data_ptr(), need), index)
+    else:
+        _run(call, pack(*args, 0, 0), index)
     return y
 
 
@@ -222,24 +286,23 @@ def paged_decode(q, seq_lens, r, w, k_pages, v_pages, block_table, k_scales=None
     `max_window` (the largest w) and num_ctas only set how the work is shared out."""
     if q.dim() != 3:
         raise ValueError("q must be (B, H, D)")
-    if k_pages.dtype != torch.int8:
-        desc, code, H, D = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
-        B, dev = q.shape[0], k_pages.device
+    if k_pages.dtype is not torch.int8:
+        index, code, shape, _, _ = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
+        B, H, D = q.shape[0], shape[1], shape[3]
         if q.shape[1:] != (H, D):
             raise ValueError(f"q must have shape {(B, H, D)}, got {tuple(q.shape)}")
-        if q.dtype != k_pages.dtype:
+        if q.dtype is not k_pages.dtype:
             raise TypeError(f"q is {q.dtype}, the cache {k_pages.dtype}")
         _table_batch(block_table, B)
-        _same_device(dev, q)
-        seq_lens = _per_seq(seq_lens, B, dev, "seq_lens")
-        r, w = _head_params(r, w, H, dev)
-        table = block_table.shape[1] * k_pages.shape[2]
-        keys = table if not max_window or max_window <= 0 else min(int(-(-max_window // 1)), table)
+        _same_device(index, q)
+        seq_lens = _per_seq(seq_lens, B, index, "seq_lens")
+        r, w = _head_params(r, w, H, index)
+        keys = _keys_seen(max_window, block_table, shape[2])
         if num_ctas is None:
             num_ctas = _tree_ctas(B * H, keys)
         # splits of every (sequence, head), at least a page each
-        num_splits = max(1, min(-(-num_ctas // max(1, B * H)), -(-keys // k_pages.shape[2])))
-        with torch.cuda.device(dev):
+        num_splits = max(1, min(-(-num_ctas // max(1, B * H)), -(-keys // shape[2])))
+        with torch.cuda.device(index):
             return _lib.screen_decode(q.detach(), seq_lens, r, w, k_pages, v_pages, block_table,
                                       eps, num_splits)[0]
     return _tree("screen_paged_decode_i8", q.unsqueeze(1), None, None, seq_lens, None, r, w, k_pages,
@@ -276,33 +339,29 @@ def paged_commit(lens, path, counts, k_pages, v_pages, block_table, k_scales=Non
     ndim = k_pages.dim()
     if ndim not in (4, 5):
         raise ValueError("pages must be [num_pages, H, page_size, D], or that per layer")
-    desc, code, H, D = _pages(k_pages, v_pages, block_table, k_scales, v_scales, ndim)
-    dev = k_pages.device
+    index, code, shape, cache, scales = _pages(k_pages, v_pages, block_table, k_scales, v_scales, ndim)
     B = block_table.shape[0]
     if path.dim() != 2 or path.shape[1] > MAX_NODES:
         raise ValueError(f"path must be (B, n) with n <= {MAX_NODES}")
     n = path.shape[1]
-    path = _node_ints(path, B, n, dev, "path")
-    lens, counts = _per_seq(lens, B, dev, "lens"), _per_seq(counts, B, dev, "counts")
-    L = k_pages.shape[0] if ndim == 5 else 1
-    if k_pages.numel() == 0 or n == 0:
+    path = _node_ints(path, B, n, index, "path")
+    lens, counts = _per_seq(lens, B, index, "lens"), _per_seq(counts, B, index, "counts")
+    P, H, ps, D = shape[-4:]
+    L = shape[0] if ndim == 5 else 1
+    if L * P * H * ps * D == 0 or n == 0:
         return
-    a = _lib.CommitArgs(cache_dtype=code, L=L, B=B, H=H, D=D, n=n, lens=lens.data_ptr(),
-                        path=path.data_ptr(), path_sb=path.stride(0), counts=counts.data_ptr(),
-                        cache=desc, k_scales=_lib._ptr(k_scales), v_scales=_lib._ptr(v_scales),
-                        layer_stride=k_pages.numel() // (L * D))
-    _run(_lib.load().screen_paged_commit, a, dev)
+    pack, call = _entry("screen_paged_commit")
+    _run(call, pack(code, L, B, H, D, n, lens.data_ptr(), path.data_ptr(), path.stride(0),
+                    counts.data_ptr(), *cache, *scales, P * H * ps), index)
 
 
-def _logit_rows(x, B, n, V, dev, name):
-    _lib._require_cuda(x)
-    _same_device(dev, x)
-    if x.shape != (B, n, V):
-        raise ValueError(f"{name} must have shape {(B, n, V)}, got {tuple(x.shape)}")
-    x = x.detach()
-    if x.dtype == torch.float16:
-        x = x.float()
-    return x if x.stride(2) == 1 or x.numel() == 0 else x.contiguous()
+def _logit_rows(x, shape, index, name):
+    _same_device(index, x)
+    if x.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
+    if x.dtype is torch.float16:
+        x = x.detach().float()
+    return x if x.stride(2) == 1 or x.numel() == 0 else x.detach().contiguous()
 
 
 def verify_drafts(logits, tokens, parents, uniforms, draft_logits=None, temperature=1.0):
@@ -329,56 +388,57 @@ def verify_drafts(logits, tokens, parents, uniforms, draft_logits=None, temperat
     entries have probability 0.  float16 logits are read as float32."""
     if logits.dim() != 3 or logits.shape[1] < 1 or logits.shape[2] < 1:
         raise ValueError("logits must be (B, n + 1, V)")
-    B, n, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    B, rows, V = logits.shape
+    n = rows - 1
     if n > MAX_NODES:
         raise ValueError(f"a tree has at most {MAX_NODES} nodes, got {n}")
-    _lib._require_cuda(logits, tokens, uniforms)
-    dev = logits.device
-    logits = _logit_rows(logits, B, n + 1, V, dev, "logits")
-    if tokens.dtype != torch.int64 or tokens.shape != (B, n):
+    index = logits.get_device()
+    if index < 0:
+        _lib._require_cuda(logits)
+    logits = _logit_rows(logits, (B, rows, V), index, "logits")
+    if tokens.dtype is not torch.int64 or tokens.shape != (B, n):
         raise ValueError(f"tokens must be int64 of shape ({B}, {n})")
-    if uniforms.dtype != torch.float32 or uniforms.shape != (B, n + 1):
-        raise ValueError(f"uniforms must be float32 of shape ({B}, {n + 1})")
-    _same_device(dev, tokens, uniforms)
-    parents = _node_ints(parents, B, n, dev, "parents")
+    if uniforms.dtype is not torch.float32 or uniforms.shape != (B, rows):
+        raise ValueError(f"uniforms must be float32 of shape ({B}, {rows})")
+    _same_device(index, tokens, uniforms)
+    parents = _node_ints(parents, B, n, index, "parents")
     if n and tokens.stride(1) != 1:
         tokens = tokens.contiguous()
     if uniforms.stride(1) != 1:
         uniforms = uniforms.contiguous()
-    a = _lib.VerifyArgs(dtype=_lib._dtype_code(logits), B=B, n=n, V=V, logits=logits.data_ptr(),
-                        l_sb=logits.stride(0), l_st=logits.stride(1), tokens=tokens.data_ptr(),
-                        t_sb=tokens.stride(0), uniforms=uniforms.data_ptr(),
-                        u_sb=uniforms.stride(0))
+    tp = 0
     if isinstance(temperature, torch.Tensor):
-        _lib._require_cuda(temperature)
-        _same_device(dev, temperature)
-        if temperature.dtype != torch.float32 or temperature.shape != (B,):
+        _same_device(index, temperature)
+        if temperature.dtype is not torch.float32 or temperature.shape != (B,):
             raise ValueError(f"temperature must be a float or float32 of shape ({B},)")
-        temperature = temperature.contiguous()
-        a.temperatures = temperature.data_ptr()
+        temps = temperature.contiguous()
+        tp, temperature = temps.data_ptr(), 1.0
     else:
         temperature = float(temperature)
         if not 0.0 <= temperature < 3.0e38:
             raise ValueError(f"temperature must be finite and not negative, got {temperature}")
-        a.temperature = temperature
+    dp = d_sb = d_st = 0
     if draft_logits is not None and n:
-        draft_logits = _logit_rows(draft_logits, B, n, V, dev, "draft_logits")
-        if draft_logits.dtype != logits.dtype:
+        draft_logits = _logit_rows(draft_logits, (B, n, V), index, "draft_logits")
+        if draft_logits.dtype is not logits.dtype:
             raise TypeError("logits and draft_logits must share a dtype")
-        a.draft_logits, a.d_sb, a.d_st = (draft_logits.data_ptr(), draft_logits.stride(0),
-                                          draft_logits.stride(1))
-    if parents is not None:
-        a.parents, a.p_sb = parents.data_ptr(), parents.stride(0)
-    out = torch.empty((B, n + 1), dtype=torch.int64, device=dev)
-    path = torch.empty((B, n), dtype=torch.int32, device=dev)
-    counts = torch.empty((B,), dtype=torch.int32, device=dev)
+        dp, (d_sb, d_st, _) = draft_logits.data_ptr(), draft_logits.stride()
+    dcode = _lib._dtype_code(logits)
+    # one allocation for the three results: int64 tokens, int32 path and counts
+    buf = tokens.new_empty(B * rows + (B * n + B + 1) // 2)
+    out = buf[:B * rows].view(B, rows)
+    small = buf[B * rows:].view(torch.int32)
+    path, counts = small[:B * n].view(B, n), small[B * n:B * n + B]
     if B == 0:
         return out, path, counts
-    a.out_tokens, a.path, a.counts = out.data_ptr(), path.data_ptr(), counts.data_ptr()
-    lib = _lib.load()
-    need = lib.screen_verify_workspace_size(ctypes.byref(a))
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    _run(lib.screen_verify_drafts, a, dev)
+    pack, call = _entry("screen_verify_drafts")
+    l_sb, l_st, _ = logits.stride()
+    pp, p_sb = (0, 0) if parents is None else (parents.data_ptr(), parents.stride(0))
+    ints = buf.data_ptr() + 8 * B * rows
+    args = (dcode, B, n, V, temperature, 0, tp, logits.data_ptr(), l_sb, l_st, dp, d_sb, d_st,
+            tokens.data_ptr() if n else 0, tokens.stride(0), pp, p_sb, uniforms.data_ptr(),
+            uniforms.stride(0), buf.data_ptr(), ints if n else 0, ints + 4 * B * n)
+    need = _size_query("screen_verify_workspace_size")(pack(*args, 0, 0))
+    ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    _run(call, pack(*args, ws.data_ptr() if need else 0, need), index)
     return out, path, counts
