@@ -164,6 +164,13 @@ def _rows(x, shape, index, name):
     return x, p, sb, st
 
 
+def _like(x, shape):
+    """A contiguous tensor of `shape`, which is x's (empty_like keeps x's order of
+    strides; it is the cheapest allocation there is)."""
+    y = torch.empty_like(x)
+    return y if y.is_contiguous() else x.new_empty(shape)
+
+
 def _table_batch(block_table, B):
     if block_table.shape[0] != B:
         raise ValueError(f"block_table has {block_table.shape[0]} rows for a batch of {B}")
@@ -235,13 +242,25 @@ def _keys_seen(max_window, block_table, page_size):
 
 def _tree(name, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_scales, v_scales,
           max_window, num_ctas, eps):
+    """q, k, v (B, n, H, D); or q (B, H, D), one query per sequence."""
     index, code, shape, cache, scales = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
-    if q.dim() != 4:
-        raise ValueError("q must be (B, n, H, D)")
-    B, n = q.shape[:2]
     H, D = shape[1], shape[3]
-    full = (B, n, H, D)
-    q, qp, q_sb, q_st = _rows(q, full, index, "q")
+    if q.dim() == 3:
+        B, n = q.shape[0], 1
+        full = (B, H, D)
+        if q.get_device() != index:
+            _same_device(index, q)
+        if q.shape != full:
+            raise ValueError(f"q must have shape {full}, got {tuple(q.shape)}")
+        q_sb, sh, sd = q.stride()
+        if sd != 1 or sh != D or q_sb % (8 if q.dtype is torch.bfloat16 else 4) or q.data_ptr() % 16:
+            q = q.detach().contiguous()
+            q_sb = H * D
+        qp, q_st = q.data_ptr(), 0
+    else:
+        B, n = q.shape[:2]
+        full = (B, n, H, D)
+        q, qp, q_sb, q_st = _rows(q, full, index, "q")
     dtype = q.dtype
     if code != _lib.I8 and dtype is not k_pages.dtype:
         raise TypeError(f"q is {q.dtype}, the cache {k_pages.dtype}")
@@ -259,7 +278,7 @@ def _tree(name, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_s
             raise TypeError("q, k, v must share a dtype")
         k, kp, k_sb, k_st = _rows(k, full, index, "k")
         v, vp, v_sb, v_st = _rows(v, full, index, "v")
-    y = q.new_empty(full)
+    y = _like(q, full)
     dcode = _lib._dtype_code(q)
     if B * n * H == 0:
         return y
@@ -272,7 +291,7 @@ def _tree(name, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_s
             y.data_ptr())
     if num_ctas > 1:
         need = _size_query("screen_tree_workspace_size")(pack(*args, 0, 0))
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = torch.UntypedStorage(need, device=q.device)
         _run(call, pack(*args, ws.data_ptr(), need), index)
     else:
         _run(call, pack(*args, 0, 0), index)
@@ -305,8 +324,8 @@ def paged_decode(q, seq_lens, r, w, k_pages, v_pages, block_table, k_scales=None
         with torch.cuda.device(index):
             return _lib.screen_decode(q.detach(), seq_lens, r, w, k_pages, v_pages, block_table,
                                       eps, num_splits)[0]
-    return _tree("screen_paged_decode_i8", q.unsqueeze(1), None, None, seq_lens, None, r, w, k_pages,
-                 v_pages, block_table, k_scales, v_scales, max_window, num_ctas, eps).squeeze(1)
+    return _tree("screen_paged_decode_i8", q, None, None, seq_lens, None, r, w, k_pages, v_pages,
+                 block_table, k_scales, v_scales, max_window, num_ctas, eps)
 
 
 def paged_tree_decode(q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_scales=None,
@@ -326,6 +345,8 @@ def paged_tree_decode(q, k, v, lens, parents, r, w, k_pages, v_pages, block_tabl
     ring table must hold ceil(max w) - 1 + n rows per sequence; nodes whose row
     falls outside the table are not seen.  `max_window` and num_ctas as in
     paged_decode."""
+    if q.dim() != 4:
+        raise ValueError("q must be (B, n, H, D)")
     return _tree("screen_tree_decode", q, k, v, lens, parents, r, w, k_pages, v_pages, block_table,
                  k_scales, v_scales, max_window, num_ctas, eps)
 
@@ -424,21 +445,20 @@ def verify_drafts(logits, tokens, parents, uniforms, draft_logits=None, temperat
             raise TypeError("logits and draft_logits must share a dtype")
         dp, (d_sb, d_st, _) = draft_logits.data_ptr(), draft_logits.stride()
     dcode = _lib._dtype_code(logits)
-    # one allocation for the three results: int64 tokens, int32 path and counts
-    buf = tokens.new_empty(B * rows + (B * n + B + 1) // 2)
-    out = buf[:B * rows].view(B, rows)
-    small = buf[B * rows:].view(torch.int32)
-    path, counts = small[:B * n].view(B, n), small[B * n:B * n + B]
+    out = torch.empty_like(uniforms, dtype=torch.int64)
+    if not out.is_contiguous():
+        out = uniforms.new_empty((B, rows), dtype=torch.int64)
+    path = torch.empty((B, n), dtype=torch.int32, device=logits.device)
+    counts = torch.empty(B, dtype=torch.int32, device=logits.device)
     if B == 0:
         return out, path, counts
     pack, call = _entry("screen_verify_drafts")
     l_sb, l_st, _ = logits.stride()
     pp, p_sb = (0, 0) if parents is None else (parents.data_ptr(), parents.stride(0))
-    ints = buf.data_ptr() + 8 * B * rows
     args = (dcode, B, n, V, temperature, 0, tp, logits.data_ptr(), l_sb, l_st, dp, d_sb, d_st,
             tokens.data_ptr() if n else 0, tokens.stride(0), pp, p_sb, uniforms.data_ptr(),
-            uniforms.stride(0), buf.data_ptr(), ints if n else 0, ints + 4 * B * n)
+            uniforms.stride(0), out.data_ptr(), path.data_ptr(), counts.data_ptr())
     need = _size_query("screen_verify_workspace_size")(pack(*args, 0, 0))
-    ws = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    ws = torch.UntypedStorage(need, device=logits.device) if need else None
     _run(call, pack(*args, ws.data_ptr() if need else 0, need), index)
     return out, path, counts
