@@ -31,58 +31,99 @@ __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, flo
   x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
 
-// The int8 form of a raw row x held by a group of G lanes, 4 elements a lane:
+// The int8 form of a raw row x held by a group of G lanes, E elements a lane (E a
+// multiple of 4), packed four to a word:
 //   m = round_half_even(127 x / max|x|),  scale = 1 / max(|m|, 127 eps / max|x|),
 // so scale * m is the unit form of the rounded raw row.  The integers do not
-// depend on any order of summation: max|x| is exact, a product that lands
-// within 2^-10 of a half is decided in 64 bits (127 x is exact there and a
-// correctly rounded quotient cannot cross a half), and |m|^2 <= 128 * 127^2 is
-// summed in integers.  A row with an infinity or NaN becomes m = 0, scale NaN.
-// All 32 lanes of the warp must call it.
-template <int G>
-__device__ __forceinline__ void int8_row(const float (&x)[4], float eps, char4& m, float& scale) {
+// depend on any order of summation: max|x| is exact, and |m|^2 <= 128 * 127^2 is
+// summed in integers.  For bf16 values (BF) 127 x is exact in 32 bits and the
+// quotient correctly rounded (a product with the rounded reciprocal and one
+// remainder step), which no half can cross; for fp32 a quotient so near a half
+// that 32 bits cannot tell (127 * 2^-23 at most; one in 16,000) is decided by an
+// exact comparison in 64 bits.  A row with an infinity or NaN becomes m = 0, scale
+// NaN.  All 32 lanes of the warp must call it; x is used up.
+template <int G, int E, bool BF>
+__device__ __forceinline__ void int8_row(float (&x)[E], float eps, uint32_t (&m)[E / 4],
+                                         float& scale) {
   uint32_t top = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+  for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o, G));
   const bool finite = top < 0x7f800000u;
   const float amax = __uint_as_float(top);
-  // 127 / amax overflows for the smallest rows: those take the 64-bit path
-  const bool tiny = amax < 1.0e-30f;
-  const float inv = tiny ? 0.f : 127.0f / amax;
-  int q[4];
+  float am = amax;
+  if (!(amax > 1.0e-30f && amax < 1.0e30f)) {
+    // outside the reciprocal's range: scaled by a power of two; a row of zeros
+    // or with a non-finite value becomes zeros
+    const float up = finite && top ? (amax < 1.0f ? 0x1p100f : 0x1p-100f) : 0.f;
+    am = up != 0.f ? amax * up : 1.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = up != 0.f ? x[e] * up : 0.f;
+  }
+  const float inv = 1.0f / am;
+  const float magic = 12582912.0f;   // 1.5 * 2^23: rounds to an integer in the low byte
+  float f[E];
+  if constexpr (BF) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float d = 127.0f * x[e], q = d * inv;
+      f[e] = fmaf(fmaf(-q, am, d), inv, q) + magic;
+    }
+  } else {
+    bool near = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float t = 127.0f * x[e] * inv;
+      f[e] = t + magic;
+      near = near || fabsf(t - (f[e] - magic)) > 0.5f - 0x1p-15f;
+    }
+    if (near) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float t = fabsf(127.0f * x[e] * inv), k = floorf(t);
+        if (fabsf(t - k - 0.5f) < 0x1p-15f) {
+          const double num = 127.0 * (double)fabsf(x[e]), half = ((double)k + 0.5) * (double)am;
+          const bool odd = (int)k & 1;
+          f[e] = copysignf(num > half || (num == half && odd) ? k + 1.0f : k, x[e]) + magic;
+        }
+      }
+    }
+  }
   int ss = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float t = x[e] * inv;
-    float f = rintf(t);
-    if (tiny || !(fabsf(t - f) < 0.5f - 0x1p-10f))
-      f = top && finite ? (float)rint((double)x[e] * 127.0 / (double)amax) : 0.f;
-    q[e] = finite ? (int)f : 0;
-    ss += q[e] * q[e];
+  for (int w = 0; w < E / 4; ++w) {
+    const uint32_t a = __float_as_uint(f[4 * w]), b = __float_as_uint(f[4 * w + 1]);
+    const uint32_t c = __float_as_uint(f[4 * w + 2]), d = __float_as_uint(f[4 * w + 3]);
+    m[w] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+    ss = __dp4a((int)m[w], (int)m[w], ss);
   }
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
-  // 1 / max(a, b) as min(1 / a, 1 / b): 127 eps / amax overflows for tiny rows
-  scale = finite ? fminf(1.0f / sqrtf((float)ss), amax / (127.0f * eps)) : __uint_as_float(0x7fc00000u);
-  m = make_char4((signed char)q[0], (signed char)q[1], (signed char)q[2], (signed char)q[3]);
+  // 1 / |m| by one Newton step from the approximate reciprocal root
+  const float n2 = (float)ss, y = rsqrtf(n2);
+  scale = fmaf(0.5f * y, fmaf(-n2 * y, y, 1.0f), y);
+  // |m| >= 127: only a row below eps can meet the other bound, 1 / max(a, b) as
+  // min(1 / a, 1 / b)
+  if (!(amax >= eps)) scale = top ? fminf(scale, amax / (127.0f * eps)) : 0.f;
+  if (!finite) scale = __uint_as_float(0x7fc00000u);
 }
 
 // Write the cache form of one raw row (G = D / 4 lanes, 4 elements a lane) at
 // row index `row` (< 0: nothing is written; the lanes still take part in the
-// shuffles).  E = signed char: int8 row and scale; else the unit row in E with
+// shuffles).  T: the raw row's type.  E = signed char: int8 row and scale; else
+// the unit row in E with
 // the arithmetic of kv_append_kernel.
-template <typename E, int D>
-__device__ __forceinline__ void write_cache_row(const float (&x)[4], float eps, int gl,
+template <typename E, typename T, int D>
+__device__ __forceinline__ void write_cache_row(float (&x)[4], float eps, int gl,
                                                 long long row, E* pages, float* scales) {
   constexpr int G = D / 4;
   if constexpr (sizeof(E) == 1) {
-    char4 m;
+    uint32_t m[1];
     float sc;
-    int8_row<G>(x, eps, m, sc);
+    int8_row<G, 4, sizeof(T) == 2>(x, eps, m, sc);
     if (row >= 0) {
-      *reinterpret_cast<char4*>(pages + row * D + gl * 4) = m;
+      *reinterpret_cast<uint32_t*>(pages + row * D + gl * 4) = m[0];
       if (gl == 0) scales[row] = sc;
     }
   } else {

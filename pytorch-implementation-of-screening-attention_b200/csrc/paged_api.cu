@@ -10,7 +10,14 @@ bool dim_ok(int D) { return D == 16 || D == 32 || D == 64 || D == 128; }
 bool act_ok(int t) { return t == SCREEN_F32 || t == SCREEN_BF16; }
 bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 bool al4(const void* p) { return ((uintptr_t)p & 3u) == 0; }
-bool raw_ok(const void* p, int64_t sb, int64_t st) { return al16(p) && sb % 4 == 0 && st % 4 == 0; }
+bool raw_ok(const void* p, int64_t sb, int64_t st, int vec = 4) {
+  return al16(p) && sb % vec == 0 && st % vec == 0;
+}
+// 2 B blocks of tokens in one grid dimension, a token a block at least; a block's
+// rows in 32 bits
+bool blocks_ok(long long B, long long H, long long n) {
+  return H < 65536 && 2 * B * n < (1ll << 31);
+}
 size_t round_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
 int cache_ok(const screen_kv_cache& c, int cache_dtype, const float* ks, const float* vs) {
@@ -75,7 +82,10 @@ int screen_paged_append_i8(const screen_paged_append_args* a, screen_stream_t st
   if (!a->k || !a->v || !a->positions) return SCREEN_ERR_INVALID_ARG;
   int st = cache_ok(a->cache, SCREEN_I8, a->k_scales, a->v_scales);
   if (st) return st;
-  if (!raw_ok(a->k, a->k_sb, a->k_st) || !raw_ok(a->v, a->v_sb, a->v_st)) return SCREEN_ERR_ALIGNMENT;
+  const int vec = a->dtype == SCREEN_BF16 ? 8 : 4;
+  if (!raw_ok(a->k, a->k_sb, a->k_st, vec) || !raw_ok(a->v, a->v_sb, a->v_st, vec))
+    return SCREEN_ERR_ALIGNMENT;
+  if (!blocks_ok(a->B, a->H, a->n_new)) return SCREEN_ERR_UNSUPPORTED;
   paged_append8(*a, (cudaStream_t)stream);
   return check_launch();
 }
@@ -91,6 +101,7 @@ int screen_paged_read(const screen_paged_read_args* a, screen_stream_t stream) {
   int st = cache_ok(a->cache, a->cache_dtype, a->k_scales, a->v_scales);
   if (st) return st;
   if (!al16(a->k) || !al16(a->v)) return SCREEN_ERR_ALIGNMENT;
+  if (!blocks_ok(a->B, a->H, a->n)) return SCREEN_ERR_UNSUPPORTED;
   paged_read(*a, (cudaStream_t)stream);
   return check_launch();
 }

@@ -6,78 +6,178 @@
 namespace screen {
 namespace {
 
-// ---------------------------------------------------------------------------
-// Append to int8 pages: D / 4 lanes per raw row, blockIdx.y selects K / V.
-// Bound by HBM: D * sizeof(T) bytes in, D + 4 out per row.  Consecutive row
-// groups walk n (the token) first: the int8 rows and scales of one head are
-// contiguous along a page, a raw row is a whole 128-byte line (bf16, D = 64)
-// wherever it lies.
-// ---------------------------------------------------------------------------
-template <typename T, int D>
-__global__ void __launch_bounds__(256) append8_kernel(screen_paged_append_args a) {
-  pdl_wait();
-  pdl_trigger();
-  constexpr int G = D / 4;
-  constexpr int RPB = 256 / G;
-  const long long row = (long long)blockIdx.x * RPB + threadIdx.x / G;
-  const int gl = threadIdx.x % G;
-  const long long rows = (long long)a.B * a.n_new * a.H;
-  const bool valid = row < rows;  // no early exit: the group shuffles need every lane
-  const long long rr = valid ? row : 0;
-  const long long n = rr % a.n_new;
-  const int h = (int)(rr / a.n_new % a.H);
-  const int b = (int)(rr / ((long long)a.H * a.n_new));
-  const bool isv = blockIdx.y == 1;
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (valid)
-    load4(reinterpret_cast<const T*>(isv ? a.v : a.k) + (long long)b * (isv ? a.v_sb : a.k_sb) +
-              n * (isv ? a.v_st : a.k_st) + (long long)h * D + gl * 4, x);
-  const long long dst = valid ? paged_row(a.cache, b, a.H, h, (long long)a.positions[b] + n) : -1;
-  write_cache_row<signed char, D>(x, a.eps, gl, dst,
-                                  reinterpret_cast<signed char*>(isv ? a.cache.v_pages : a.cache.k_pages),
-                                  isv ? a.v_scales : a.k_scales);
+// A block moves `tokens` consecutive tokens of one sequence, all heads, K in the
+// lower half of the grid, V in the upper.  Heads run fastest through its rows:
+// a token's raw rows are one contiguous run of H * D elements, and a few tokens
+// make a run of each head's page (walking the tokens of one head first, 128-byte
+// rows 6 KB apart, read the packed QKV projection at 0.7 TB/s).  A group of G
+// lanes moves a row 16 bytes a lane (of the wider side), R rows of a group with
+// all loads in flight before the first use.
+constexpr int kThreads = 256;
+struct RowBlock {
+  int b, n0, rows;       // rows of the block, row r: token n0 + r / H, head r % H
+  bool isv;
+};
+// r / H for r, H < 65536: inv = ceil(2^32 / H)
+__device__ __forceinline__ int div_heads(int r, int H, unsigned inv) {
+  return H == 1 ? r : (int)__umulhi((unsigned)r, inv);
+}
+__device__ __forceinline__ RowBlock row_block(int B, int H, int n, int tokens) {
+  const unsigned tiles = ((unsigned)n + tokens - 1) / tokens;
+  unsigned id = blockIdx.x;
+  RowBlock r;
+  r.isv = id >= tiles * (unsigned)B;
+  if (r.isv) id -= tiles * (unsigned)B;
+  r.b = (int)(id / tiles);
+  r.n0 = (int)((id - r.b * tiles) * tokens);
+  r.rows = min(tokens, n - r.n0) * H;
+  return r;
+}
+// paged_row() for a sequence's table row
+__device__ __forceinline__ long long table_row(const screen_kv_cache& c, const int* table, int H,
+                                               int h, long long pos) {
+  if (pos < 0 || pos > 0x7fffffff) return -1;
+  const unsigned p = (unsigned)pos, ps = (unsigned)c.page_size;
+  const unsigned blk = (ps & (ps - 1)) == 0 ? p >> (31 - __clz(ps)) : p / ps;
+  if (blk >= (unsigned)c.max_blocks) return -1;
+  const int page = table[blk];
+  if (page < 0 || page >= c.num_pages) return -1;
+  return ((long long)page * H + h) * ps + (p - blk * ps);
 }
 
 // ---------------------------------------------------------------------------
-// Read back: out (B, n, H, D) contiguous, 4 elements a lane.
+// Append to int8 pages.  Bound by HBM: D * sizeof(T) bytes in, D + 4 out per
+// row.
 // ---------------------------------------------------------------------------
-template <typename E>
-__device__ __forceinline__ void row4(const E* p, float (&x)[4]) {
-  if constexpr (sizeof(E) == 1) {
-    const char4 c = *reinterpret_cast<const char4*>(p);
-    x[0] = c.x; x[1] = c.y; x[2] = c.z; x[3] = c.w;
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, float (&x)[16 / sizeof(T)]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  if constexpr (sizeof(T) == 2) {
+    const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), d = unpack_bf16(u.w);
+    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+    x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
   } else {
-    load4(p, x);
+    x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y);
+    x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
   }
 }
-template <typename E, typename T, int D>
-__global__ void __launch_bounds__(256) paged_read_kernel(screen_paged_read_args a) {
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(kThreads) append8_kernel(screen_paged_append_args a, int tokens,
+                                                                unsigned inv_heads) {
   pdl_wait();
   pdl_trigger();
-  constexpr int G = D / 4;
-  constexpr int RPB = 256 / G;
-  const long long row = (long long)blockIdx.x * RPB + threadIdx.x / G;
-  const int gl = threadIdx.x % G;
-  if (row >= (long long)a.B * a.n * a.H) return;
-  const long long n = row % a.n;
-  const int h = (int)(row / a.n % a.H);
-  const int b = (int)(row / ((long long)a.H * a.n));
-  const bool isv = blockIdx.y == 1;
-  const long long src = paged_row(a.cache, b, a.H, h, (long long)a.positions[b] + n);
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (src >= 0) {
-    row4(reinterpret_cast<const E*>(isv ? a.cache.v_pages : a.cache.k_pages) + src * D + gl * 4, x);
-    if constexpr (sizeof(E) == 1) {
-      const float sc = (isv ? a.v_scales : a.k_scales)[src];
+  constexpr int E = 16 / (int)sizeof(T), G = D / E, GROUPS = kThreads / G;
+  const RowBlock rb = row_block(a.B, a.H, a.n_new, tokens);
+  const int gl = threadIdx.x % G, grp = threadIdx.x / G;
+  const long long sb = rb.isv ? a.v_sb : a.k_sb, st = rb.isv ? a.v_st : a.k_st;
+  const T* src = reinterpret_cast<const T*>(rb.isv ? a.v : a.k) + (long long)rb.b * sb + gl * E;
+  const int* table = a.cache.block_table + (long long)rb.b * a.cache.max_blocks;
+  const long long pos0 = a.positions[rb.b];
+  signed char* pages = reinterpret_cast<signed char*>(rb.isv ? a.cache.v_pages : a.cache.k_pages);
+  float* scales = rb.isv ? a.v_scales : a.k_scales;
+#pragma unroll 1
+  for (int r0 = 0; r0 < rb.rows; r0 += R * GROUPS) {   // uniform: the shuffles need every lane
+    float x[R][E];
+    long long row[R];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] *= sc;
+    for (int i = 0; i < R; ++i) {
+      const int r = r0 + i * GROUPS + grp;
+      row[i] = -1;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+      if (r < rb.rows) {
+        const int t = div_heads(r, a.H, inv_heads), h = r - t * a.H, n = rb.n0 + t;
+        load16(src + n * st + (long long)h * D, x[i]);
+        row[i] = table_row(a.cache, table, a.H, h, pos0 + n);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      uint32_t m[E / 4];
+      float sc;
+      int8_row<G, E, sizeof(T) == 2>(x[i], a.eps, m, sc);
+      if (row[i] >= 0) {
+        signed char* dst = pages + row[i] * D + gl * E;
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(m[0], m[1]);
+        else *reinterpret_cast<uint32_t*>(dst) = m[0];
+        if (gl == 0) scales[row[i]] = sc;
+      }
     }
   }
-  T* out = reinterpret_cast<T*>(isv ? a.v : a.k) + (((long long)b * a.n + n) * a.H + h) * D + gl * 4;
-  if constexpr (sizeof(T) == 4)
-    *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
-  else
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+}
+
+// ---------------------------------------------------------------------------
+// Read back: out (B, n, H, D) contiguous, 16 bytes of it a lane.
+// ---------------------------------------------------------------------------
+template <typename E, int N>
+__device__ __forceinline__ void row_n(const E* p, float (&x)[N]) {
+  if constexpr (sizeof(E) == 1) {
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+      const char4 c = *reinterpret_cast<const char4*>(p + 4 * w);
+      x[4 * w] = c.x; x[4 * w + 1] = c.y; x[4 * w + 2] = c.z; x[4 * w + 3] = c.w;
+    }
+  } else {
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+      float y[4];
+      load4(p + 4 * w, y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * w + e] = y[e];
+    }
+  }
+}
+template <typename E, typename T, int D, int R>
+__global__ void __launch_bounds__(kThreads) paged_read_kernel(screen_paged_read_args a, int tokens,
+                                                                   unsigned inv_heads) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int N = 16 / (int)sizeof(T), G = D / N, GROUPS = kThreads / G;
+  const RowBlock rb = row_block(a.B, a.H, a.n, tokens);
+  const int gl = threadIdx.x % G, grp = threadIdx.x / G;
+  const int* table = a.cache.block_table + (long long)rb.b * a.cache.max_blocks;
+  const long long pos0 = a.positions[rb.b];
+  const E* pages = reinterpret_cast<const E*>(rb.isv ? a.cache.v_pages : a.cache.k_pages);
+  const float* scales = rb.isv ? a.v_scales : a.k_scales;
+  T* out = reinterpret_cast<T*>(rb.isv ? a.v : a.k) + ((long long)rb.b * a.n + rb.n0) * a.H * D + gl * N;
+#pragma unroll 1
+  for (int r0 = grp; r0 < rb.rows; r0 += R * GROUPS) {
+    float x[R][N], sc[R];
+    long long row[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int r = r0 + i * GROUPS;
+      row[i] = -1;
+      if (r < rb.rows) {
+        const int t = div_heads(r, a.H, inv_heads);
+        row[i] = table_row(a.cache, table, a.H, r - t * a.H, pos0 + rb.n0 + t);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[i][e] = 0.f;
+      sc[i] = 1.f;
+      if (row[i] >= 0) {
+        row_n(pages + row[i] * D + gl * N, x[i]);
+        if constexpr (sizeof(E) == 1) sc[i] = scales[row[i]];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int r = r0 + i * GROUPS;
+      if (r >= rb.rows) continue;
+      if constexpr (sizeof(E) == 1)
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[i][e] *= sc[i];
+      T* dst = out + (long long)r * D;
+      if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4*>(dst) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+      else
+        *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(x[i][0], x[i][1]), pack_bf16(x[i][2], x[i][3]),
+                                                    pack_bf16(x[i][4], x[i][5]), pack_bf16(x[i][6], x[i][7]));
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -137,18 +237,31 @@ __global__ void __launch_bounds__(128) commit_kernel(screen_commit_args a, int r
       if (to_s[i] >= 0) scales[to_s[i]] = sc_s[i];
 }
 
+// Tokens of a block: as many as its groups hold at R rows each.
+struct RowGrid {
+  int tokens;
+  unsigned blocks, inv_heads;
+};
+RowGrid row_grid(int B, int H, int n, int rows) {
+  RowGrid g;
+  g.tokens = rows > H ? rows / H : 1;
+  g.inv_heads = (unsigned)(((1ull << 32) + H - 1) / H);
+  g.blocks = 2u * B * (unsigned)((n + g.tokens - 1) / g.tokens);
+  return g;
+}
 template <typename T, int D>
 void launch_append8(const screen_paged_append_args& a, cudaStream_t s) {
-  constexpr int RPB = 256 / (D / 4);
-  const long long rows = (long long)a.B * a.n_new * a.H;
-  launch_pdl(append8_kernel<T, D>, dim3((unsigned)((rows + RPB - 1) / RPB), 2), dim3(256), 0, s, a);
+  constexpr int R = 4, GROUPS = kThreads / (D * (int)sizeof(T) / 16);
+  const RowGrid g = row_grid(a.B, a.H, a.n_new, R * GROUPS);
+  launch_pdl(append8_kernel<T, D, R>, dim3(g.blocks), dim3(kThreads), 0, s, a, g.tokens,
+             g.inv_heads);
 }
 template <typename E, typename T, int D>
 void launch_read(const screen_paged_read_args& a, cudaStream_t s) {
-  constexpr int RPB = 256 / (D / 4);
-  const long long rows = (long long)a.B * a.n * a.H;
-  launch_pdl(paged_read_kernel<E, T, D>, dim3((unsigned)((rows + RPB - 1) / RPB), 2), dim3(256), 0,
-             s, a);
+  constexpr int R = 4, GROUPS = kThreads / (D * (int)sizeof(T) / 16);
+  const RowGrid g = row_grid(a.B, a.H, a.n, R * GROUPS);
+  launch_pdl(paged_read_kernel<E, T, D, R>, dim3(g.blocks), dim3(kThreads), 0, s, a, g.tokens,
+             g.inv_heads);
 }
 template <int D>
 void append8_d(const screen_paged_append_args& a, cudaStream_t s) {

@@ -234,7 +234,7 @@ __device__ __forceinline__ void append_rows(const screen_tree_args& a, const Nod
       load4(reinterpret_cast<const TA*>(isv ? a.v : a.k) + (long long)b * (isv ? a.v_sb : a.k_sb) +
                 (long long)i * (isv ? a.v_st : a.k_st) + (long long)h * D + gl * 4, x);
     const long long row = take ? paged_row(a.cache, b, a.H, h, lens + i) : -1;
-    write_cache_row<E, D>(x, a.eps, gl, row,
+    write_cache_row<E, TA, D>(x, a.eps, gl, row,
                           reinterpret_cast<E*>(isv ? a.cache.v_pages : a.cache.k_pages),
                           isv ? a.v_scales : a.k_scales);
   }
