@@ -138,10 +138,16 @@ __device__ __forceinline__ void load_k(const unsigned char* kt, int r, int t,
       w[0] = *reinterpret_cast<const uint32_t*>(kt + r * C::RB + 4 * t);
     }
 #pragma unroll
+    for (int s = 0; s < W; ++s) w[s] ^= 0x80808080u;
+#pragma unroll
     for (int s = 0; s < W; ++s) {
-      const uint32_t u = w[s] ^ 0x80808080u;
-      kb[s][0] = f16_of_biased(__byte_perm(u, 0x64646464u, 0x4140));
-      kb[s][1] = f16_of_biased(__byte_perm(u, 0x64646464u, 0x4342));
+      kb[s][0] = __byte_perm(w[s], 0x64646464u, 0x4140);
+      kb[s][1] = __byte_perm(w[s], 0x64646464u, 0x4342);
+    }
+#pragma unroll
+    for (int s = 0; s < W; ++s) {
+      kb[s][0] = f16_of_biased(kb[s][0]);
+      kb[s][1] = f16_of_biased(kb[s][1]);
     }
   } else if constexpr (C::D >= 32) {
 #pragma unroll
@@ -170,38 +176,50 @@ __device__ __forceinline__ void load_v(const unsigned char* vt, int base, int la
                                        uint32_t (&vb)[C::NT][2]) {
   const int g = lane >> 2, t = lane & 3;
   if constexpr (C::I8) {
+    constexpr int W = C::NT >= 4 ? C::NT / 4 : 1;
+    uint32_t x[2][W], y[2][W];            // rows of a thread's key pair, both halves
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {      // keys 0-7 / 8-15 of the group
       const int r0 = base + 8 * hh + key_of<C>(2 * t), r1 = base + 8 * hh + key_of<C>(2 * t + 1);
-      constexpr int W = C::NT >= 4 ? C::NT / 4 : 1;
-      uint32_t x[W], y[W];
       if constexpr (C::D == 128) {
-        *reinterpret_cast<uint4*>(&x[0]) = *reinterpret_cast<const uint4*>(vt + v_off<C>(r0, g));
-        *reinterpret_cast<uint4*>(&y[0]) = *reinterpret_cast<const uint4*>(vt + v_off<C>(r1, g));
+        *reinterpret_cast<uint4*>(&x[hh][0]) = *reinterpret_cast<const uint4*>(vt + v_off<C>(r0, g));
+        *reinterpret_cast<uint4*>(&y[hh][0]) = *reinterpret_cast<const uint4*>(vt + v_off<C>(r1, g));
       } else if constexpr (C::D == 64) {
-        *reinterpret_cast<uint2*>(&x[0]) =
+        *reinterpret_cast<uint2*>(&x[hh][0]) =
             *reinterpret_cast<const uint2*>(vt + v_off<C>(r0, g >> 1) + 8 * (g & 1));
-        *reinterpret_cast<uint2*>(&y[0]) =
+        *reinterpret_cast<uint2*>(&y[hh][0]) =
             *reinterpret_cast<const uint2*>(vt + v_off<C>(r1, g >> 1) + 8 * (g & 1));
       } else if constexpr (C::D == 32) {
-        x[0] = *reinterpret_cast<const uint32_t*>(vt + r0 * C::RB + 4 * g);
-        y[0] = *reinterpret_cast<const uint32_t*>(vt + r1 * C::RB + 4 * g);
+        x[hh][0] = *reinterpret_cast<const uint32_t*>(vt + r0 * C::RB + 4 * g);
+        y[hh][0] = *reinterpret_cast<const uint32_t*>(vt + r1 * C::RB + 4 * g);
       } else {
-        x[0] = *reinterpret_cast<const unsigned short*>(vt + r0 * C::RB + 2 * g);
-        y[0] = *reinterpret_cast<const unsigned short*>(vt + r1 * C::RB + 2 * g);
-      }
-#pragma unroll
-      for (int q = 0; q < W; ++q) {
-        const uint32_t lo = __byte_perm(x[q], y[q], 0x5140) ^ 0x80808080u;  // x0 y0 x1 y1
-        vb[4 * q + 0][hh] = f16_of_biased(__byte_perm(lo, 0x64646464u, 0x4140));
-        vb[4 * q + 1][hh] = f16_of_biased(__byte_perm(lo, 0x64646464u, 0x4342));
-        if constexpr (C::NT >= 4) {
-          const uint32_t hi = __byte_perm(x[q], y[q], 0x7362) ^ 0x80808080u;
-          vb[4 * q + 2][hh] = f16_of_biased(__byte_perm(hi, 0x64646464u, 0x4140));
-          vb[4 * q + 3][hh] = f16_of_biased(__byte_perm(hi, 0x64646464u, 0x4342));
-        }
+        x[hh][0] = *reinterpret_cast<const unsigned short*>(vt + r0 * C::RB + 2 * g);
+        y[hh][0] = *reinterpret_cast<const unsigned short*>(vt + r1 * C::RB + 2 * g);
       }
     }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int q = 0; q < W; ++q) {
+        const uint32_t lo = __byte_perm(x[hh][q], y[hh][q], 0x5140);   // x0 y0 x1 y1
+        y[hh][q] = __byte_perm(x[hh][q], y[hh][q], 0x7362) ^ 0x80808080u;   // x2 y2 x3 y3
+        x[hh][q] = lo ^ 0x80808080u;
+      }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int q = 0; q < W; ++q) {
+        vb[4 * q + 0][hh] = __byte_perm(x[hh][q], 0x64646464u, 0x4140);
+        vb[4 * q + 1][hh] = __byte_perm(x[hh][q], 0x64646464u, 0x4342);
+        if constexpr (C::NT >= 4) {
+          vb[4 * q + 2][hh] = __byte_perm(y[hh][q], 0x64646464u, 0x4140);
+          vb[4 * q + 3][hh] = __byte_perm(y[hh][q], 0x64646464u, 0x4342);
+        }
+      }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j) vb[j][hh] = f16_of_biased(vb[j][hh]);
   } else {
     // ldmatrix.trans: lanes 0-7 / 8-15 address keys 0-7 / 8-15 of chunk c, lanes
     // 16-31 those of chunk c + 1
@@ -506,22 +524,35 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
                     else
                       mma_b16(c[nt][m], qa[m][x2], kb[nt][x2][0], kb[nt][x2][1]);
                   }
+              // step by step over all scores: their chains run side by side
 #pragma unroll
               for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                 for (int m = 0; m < QW; ++m)
 #pragma unroll
                   for (int e = 0; e < RH; ++e) {
-                    float2 v = make_float2(c[nt][m][2 * e], c[nt][m][2 * e + 1]);
+                    s[m][nt][e] = make_float2(c[nt][m][2 * e], c[nt][m][2 * e + 1]);
                     if constexpr (C::QHL) {
-                      v.x += d[nt][m][2 * e];
-                      v.y += d[nt][m][2 * e + 1];
+                      s[m][nt][e].x += d[nt][m][2 * e];
+                      s[m][nt][e].y += d[nt][m][2 * e + 1];
                     }
-                    if constexpr (C::I8) v = mul2(v, ks[nt]);
-                    v = fma2(v, both(rq[m][e]), one_r);
-                    // NaN (an unseen row, a non-finite key) counts as 0
-                    s[m][nt][e] = make_float2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f));
+                    if constexpr (C::I8) s[m][nt][e] = mul2(s[m][nt][e], ks[nt]);
                   }
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int m = 0; m < QW; ++m)
+#pragma unroll
+                  for (int e = 0; e < RH; ++e)
+                    s[m][nt][e] = fma2(s[m][nt][e], both(rq[m][e]), one_r);
+              // NaN (an unseen row, a non-finite key) counts as 0
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int m = 0; m < QW; ++m)
+#pragma unroll
+                  for (int e = 0; e < RH; ++e)
+                    s[m][nt][e] = make_float2(fmaxf(s[m][nt][e].x, 0.f), fmaxf(s[m][nt][e].y, 0.f));
             }
             if (edge) {
 #pragma unroll
@@ -594,51 +625,84 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
                 hc[nt] = mul2(vs, both(0x1p19f));
               }
             }
+            float2 al[QW][2][RH];
 #pragma unroll
-            for (int m = 0; m < QW; ++m) {
-              uint32_t pa[4] = {0u, 0u, 0u, 0u}, pl[4] = {0u, 0u, 0u, 0u};
+            for (int m = 0; m < QW; ++m)
 #pragma unroll
               for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                for (int e = 0; e < RH; ++e) {
-                  const float2 x1 = s[m][nt][e];
-                  const float2 mk = fma2(cc[nt], both(ci[m][e]), fma2(sc[nt], both(si[m][e]), hc[nt]));
-                  float2 al = mul2(mul2(x1, x1), mk);
-                  if (bad) {
+                for (int e = 0; e < RH; ++e) al[m][nt][e] = fma2(sc[nt], both(si[m][e]), hc[nt]);
+#pragma unroll
+            for (int m = 0; m < QW; ++m)
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int e = 0; e < RH; ++e) al[m][nt][e] = fma2(cc[nt], both(ci[m][e]), al[m][nt][e]);
+#pragma unroll
+            for (int m = 0; m < QW; ++m)
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int e = 0; e < RH; ++e)
+                  al[m][nt][e] = mul2(mul2(s[m][nt][e], s[m][nt][e]), al[m][nt][e]);
+            if (bad) {
+#pragma unroll
+              for (int m = 0; m < QW; ++m)
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                  for (int e = 0; e < RH; ++e) {
                     const uint32_t two = bad >> (8 * nt + 2 * t);
+                    const float2 x1 = s[m][nt][e];
                     if (((two & 1) && x1.x > 0.f) || ((two & 2) && x1.y > 0.f))
                       o[m][0][2 * e] = __uint_as_float(0x7fc00000u);
-                    if (two & 1) al.x = 0.f;
-                    if (two & 2) al.y = 0.f;
+                    if (two & 1) al[m][nt][e].x = 0.f;
+                    if (two & 2) al[m][nt][e].y = 0.f;
                   }
+            }
+            // a fragment's registers: row half e of 8-key tile nt
+            uint32_t pa[QW][4], pl[C::PHL ? QW : 1][4];
+#pragma unroll
+            for (int m = 0; m < QW; ++m)
+#pragma unroll
+              for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
                   const int f = 2 * nt + e;
-                  if constexpr (C::I8) {
-                    pa[f] = pack_f16(al.x, al.y);
-                    if constexpr (C::PHL) {
-                      const float2 u = __half22float2(*reinterpret_cast<__half2*>(&pa[f]));
-                      pl[f] = pack_f16(al.x - u.x, al.y - u.y);
-                    }
-                  } else {
-                    pa[f] = pack_bf16(al.x, al.y);
-                    const float2 u = unpack_bf16(pa[f]);
-                    pl[f] = pack_bf16(al.x - u.x, al.y - u.y);
+                  if (e >= RH) {
+                    pa[m][f] = 0u;
+                    if constexpr (C::PHL) pl[m][f] = 0u;
+                    continue;
+                  }
+                  const float2 v = al[m][nt][e < RH ? e : 0];
+                  pa[m][f] = C::I8 ? pack_f16(v.x, v.y) : pack_bf16(v.x, v.y);
+                  if constexpr (C::PHL) {
+                    const float2 u = C::I8 ? __half22float2(*reinterpret_cast<__half2*>(&pa[m][f]))
+                                           : unpack_bf16(pa[m][f]);
+                    pl[m][f] = C::I8 ? pack_f16(v.x - u.x, v.y - u.y) : pack_bf16(v.x - u.x, v.y - u.y);
                   }
                 }
+#pragma unroll
+            for (int m = 0; m < QW; ++m)
 #pragma unroll
               for (int j = 0; j < C::NT; ++j) {
                 if constexpr (C::QHL) {
                   float d[4] = {0.f, 0.f, 0.f, 0.f};
-                  mma_f16(d, pl, vb[j][0], vb[j][1]);
-                  mma_f16(d, pa, vb[j][0], vb[j][1]);
+                  mma_f16(d, pl[m], vb[j][0], vb[j][1]);
+                  mma_f16(d, pa[m], vb[j][0], vb[j][1]);
 #pragma unroll
                   for (int f = 0; f < 2 * RH; ++f) o[m][j][f] += d[f];
                 } else if constexpr (C::I8) {
-                  mma_f16(o[m][j], pa, vb[j][0], vb[j][1]);
+                  mma_f16(o[m][j], pa[m], vb[j][0], vb[j][1]);
                 } else {
-                  mma_b16(o[m][j], pa, vb[j][0], vb[j][1]);
-                  mma_b16(o[m][j], pl, vb[j][0], vb[j][1]);
+                  mma_b16(o[m][j], pl[m], vb[j][0], vb[j][1]);
                 }
               }
+            if constexpr (!C::I8) {
+#pragma unroll
+              for (int m = 0; m < QW; ++m)
+#pragma unroll
+                for (int j = 0; j < C::NT; ++j) mma_b16(o[m][j], pa[m], vb[j][0], vb[j][1]);
             }
           }
         }
