@@ -22,6 +22,20 @@ __device__ __forceinline__ void mma_b16(float* c, const uint32_t* a, uint32_t b0
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The first product of a chain: sums from zero, no registers cleared for it.
+template <bool F16>
+__device__ __forceinline__ void mma_first(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -76,7 +90,9 @@ struct Cfg {
   static constexpr int S = CONV ? 4 : RB * KT <= 2048 ? 3 : 2;   // stages of a group's ring
   static constexpr int RING_B = S * STAGE_B;
   static constexpr int HALF_B = CONV ? KT * D_ * 2 : 0;   // fp16 tile; K and V, two of each
-  static constexpr int GROUP_B = RING_B + 4 * HALF_B;
+  static constexpr int PLAN_B = MG_ > 1 ? 2 * (KT + 1) * 8 + 16 : 0;   // see `plan`; two of them
+  static constexpr int PLAN_AT = RING_B + 4 * HALF_B;
+  static constexpr int GROUP_B = (PLAN_AT + PLAN_B + 15) / 16 * 16;
   static constexpr int RED_B = 4 * 16 * D_ * 4;       // the warps' sums at the end
   static constexpr int SMEM = WK * GROUP_B > RED_B ? WK * GROUP_B : RED_B;
   // CTAs per SM the registers are cut to: what a thread holds of O and q decides
@@ -317,29 +333,49 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
       if (page < 0 || page >= a.cache.num_pages) return -1;
       return ((long long)page * a.H + h) * ps + (q - blk * (unsigned)ps);
     };
-    auto load_stage = [&](int x, int slot, long long row) {
+    // In a group of several warps they take turns in looking a stage's rows up: its
+    // warp leaves them in a plan (rows, then the first row if all follow it, else
+    // -1) that the group reads after its next barrier.
+    auto plan = [&](int turn) {
+      return reinterpret_cast<long long*>(ring + C::PLAN_AT) + (turn & 1) * (KT + 1);
+    };
+    auto first_of_run = [&](long long row) -> long long {
+      const long long row0 = __shfl_sync(0xffffffffu, row, 0);
+      const bool run = __all_sync(0xffffffffu, lane >= KT || row == row0 + lane) && row0 >= 0;
+      return run ? row0 : -1;
+    };
+    auto make_plan = [&](int turn, long long row) {
+      const long long row0 = first_of_run(row);
+      long long* pl = plan(turn);
+      if (lane < KT) pl[lane] = row;
+      if (lane == 0) pl[KT] = row0;
+    };
+    // `row`: this lane's key, of the warp whose turn it is
+    auto load_stage = [&](int turn, int slot, long long row, bool planned) {
+      const int x = s0 + wk + turn * C::WK;
       unsigned char* st = ring + (size_t)slot * C::STAGE_B;
       if (x <= s1) {
         const uint32_t sa = smem_u32(st);
         const char* kp = reinterpret_cast<const char*>(a.cache.k_pages);
         const char* vp = reinterpret_cast<const char*>(a.cache.v_pages);
-        const long long row0 = __shfl_sync(0xffffffffu, row, 0);
-        const bool run = __all_sync(0xffffffffu, lane >= KT || row == row0 + lane) && row0 >= 0;
-        if (run) {                                     // all keys there, one after another
+        const long long* pl = plan(turn);
+        const long long row0 = C::MG > 1 && planned ? pl[KT] : first_of_run(row);
+        if (row0 >= 0) {                               // all keys there, one after another
+          const long long off = row0 * C::RB + gt * 16;
 #pragma unroll
           for (int i = 0; i < (KT * C::CH + GT - 1) / GT; ++i) {
             const int u = i * GT + gt;
             if (KT * C::CH % GT == 0 || u < KT * C::CH) {
-              const long long off = row0 * C::RB + u * 16;
-              cp_async16(sa + k_off<C>(u / C::CH, u % C::CH), kp + off, true);
-              cp_async16(sa + C::TILE_B + v_off<C>(u / C::CH, u % C::CH), vp + off, true);
+              cp_async16(sa + k_off<C>(u / C::CH, u % C::CH), kp + off + i * GT * 16, true);
+              cp_async16(sa + C::TILE_B + v_off<C>(u / C::CH, u % C::CH), vp + off + i * GT * 16, true);
             }
           }
         } else {
 #pragma unroll 1
           for (int i = 0; i < (KT * C::CH + GT - 1) / GT; ++i) {
             const int u = i * GT + gt, k = u / C::CH;
-            const long long at = __shfl_sync(0xffffffffu, row, k & (KT - 1));
+            long long at = __shfl_sync(0xffffffffu, row, k & (KT - 1));
+            if (C::MG > 1 && planned) at = pl[k & (KT - 1)];
             if (k < KT) {
               const long long off = (at < 0 ? 0 : at) * C::RB + u % C::CH * 16;
               cp_async16(sa + k_off<C>(k, u % C::CH), kp + off, at >= 0);
@@ -347,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
             }
           }
         }
-        if (mg == 0) {
+        if (mg == turn % C::MG) {
           // this lane's key, stored at its score column
           const int k = lane & (KT - 1);
           const int col = (k & ~7) | key_of<C>(k & 7); // key_of is its own inverse
@@ -399,6 +435,14 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
           *reinterpret_cast<uint4*>(kh + C::HALF_B + off16<C::CH16>(k, 2 * c)) = y0;
           *reinterpret_cast<uint4*>(kh + C::HALF_B + off16<C::CH16>(k, 2 * c + 1)) = y1;
         }
+      }
+      // the mask's factors with the V row's scale in them, once for all warps
+      if (gt < KT) {
+        float* cs = reinterpret_cast<float*>(ring + (size_t)slot * C::STAGE_B + 2 * C::TILE_B) + gt;
+        const float vs = cs[3 * KT];
+        cs[0] *= vs;
+        cs[KT] *= vs;
+        cs[3 * KT] = vs * 0x1p19f;
       }
     };
 
@@ -506,13 +550,14 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
 #pragma unroll
         for (int f = 0; f < 4; ++f) o[j][f] = 0.f;
       if (rg.any) {
-        // stage x of the group sits in ring slot (its turn) % S
+        // the group's stage number `turn` sits in ring slot turn % S
         long long rows[S - 1], next;
 #pragma unroll
         for (int i = 0; i < S - 1; ++i) rows[i] = key_row(s0 + wk + i * C::WK);
         next = key_row(s0 + wk + (S - 1) * C::WK);
 #pragma unroll
-        for (int i = 0; i < S - 1; ++i) load_stage(s0 + wk + i * C::WK, i, rows[i]);
+        for (int i = 0; i < S - 1; ++i) load_stage(i, i, rows[i], false);
+        if (C::MG > 1 && mg == (S - 1) % C::MG) make_plan(S - 1, next);
         int slot = 0, fill = S - 1, buf = 0;
         if constexpr (C::CONV) {
           cp_async_wait<S - 2>();
@@ -520,11 +565,14 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
           if (s0 + wk <= s1) widen_stage(0, 0);
         }
 #pragma unroll 1
-        for (int x = s0 + wk; x <= s1; x += C::WK) {
+        for (int x = s0 + wk, turn = 0; x <= s1; x += C::WK, ++turn) {
           cp_async_wait<S - 2 - AHEAD>();
           group_sync();
-          load_stage(x + (S - 1) * C::WK, fill, next);
-          next = key_row(x + S * C::WK);
+          load_stage(turn + S - 1, fill, next, true);
+          if (C::MG == 1 || mg == (turn + S) % C::MG) {
+            next = key_row(x + S * C::WK);
+            if constexpr (C::MG > 1) make_plan(turn + S, next);
+          }
           const unsigned char* st = ring + (size_t)slot * C::STAGE_B;
           const float* cs = reinterpret_cast<const float*>(st + 2 * C::TILE_B);
           const int* cpos = reinterpret_cast<const int*>(cs) + (C::I8 ? 4 : 2) * KT;
@@ -543,13 +591,6 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
           float2 s[N8][RH];                            // keys 2t, 2t + 1 of an 8-key tile
           {
             float c[N8][4], d[C::QHL ? N8 : 1][4];
-#pragma unroll
-            for (int nt = 0; nt < N8; ++nt)
-#pragma unroll
-              for (int f = 0; f < 4; ++f) {
-                c[nt][f] = 0.f;
-                if constexpr (C::QHL) d[nt][f] = 0.f;
-              }
             if constexpr (C::LDM) {
 #pragma unroll
               for (int x2 = 0; x2 < C::KS; ++x2) {
@@ -560,11 +601,15 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
                 // truncate
                 if constexpr (C::QHL) {
 #pragma unroll
-                  for (int nt = 0; nt < N8; ++nt) mma_f16(d[nt], ql[x2], kb[nt][0], kb[nt][1]);
+                  for (int nt = 0; nt < N8; ++nt) {
+                    if (x2 == 0) mma_first<true>(d[nt], ql[x2], kb[nt][0], kb[nt][1]);
+                    else mma_f16(d[nt], ql[x2], kb[nt][0], kb[nt][1]);
+                  }
                 }
 #pragma unroll
                 for (int nt = 0; nt < N8; ++nt) {
-                  if constexpr (C::I8) mma_f16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
+                  if (x2 == 0) mma_first<C::I8>(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
+                  else if constexpr (C::I8) mma_f16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
                   else mma_b16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
                 }
               }
@@ -576,12 +621,18 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
               for (int x2 = 0; x2 < C::KS; ++x2) {
                 if constexpr (C::QHL) {
 #pragma unroll
-                  for (int nt = 0; nt < N8; ++nt)
-                    mma_f16(d[nt], ql[x2], kb[nt >> 1][nt & 1][x2][0], kb[nt >> 1][nt & 1][x2][1]);
+                  for (int nt = 0; nt < N8; ++nt) {
+                    const uint32_t* k2 = kb[nt >> 1][nt & 1][x2];
+                    if (x2 == 0) mma_first<true>(d[nt], ql[x2], k2[0], k2[1]);
+                    else mma_f16(d[nt], ql[x2], k2[0], k2[1]);
+                  }
                 }
 #pragma unroll
-                for (int nt = 0; nt < N8; ++nt)
-                  mma_f16(c[nt], qa[x2], kb[nt >> 1][nt & 1][x2][0], kb[nt >> 1][nt & 1][x2][1]);
+                for (int nt = 0; nt < N8; ++nt) {
+                  const uint32_t* k2 = kb[nt >> 1][nt & 1][x2];
+                  if (x2 == 0) mma_first<true>(c[nt], qa[x2], k2[0], k2[1]);
+                  else mma_f16(c[nt], qa[x2], k2[0], k2[1]);
+                }
               }
             }
             if constexpr (C::QHL) {
@@ -648,9 +699,13 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
             float2 hc = both(0.5f);
             if constexpr (C::I8) {
               const float2 vs = *reinterpret_cast<const float2*>(cs + 3 * KT + nt * 8 + 2 * t);
-              cc = mul2(cc, vs);
-              sc = mul2(sc, vs);
-              hc = mul2(vs, both(0x1p19f));
+              if constexpr (C::CONV) {
+                hc = vs;
+              } else {
+                cc = mul2(cc, vs);
+                sc = mul2(sc, vs);
+                hc = mul2(vs, both(0x1p19f));
+              }
             }
 #pragma unroll
             for (int e = 0; e < RH; ++e) al[nt][e] = fma2(sc, both(si[e]), hc);
@@ -730,8 +785,8 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
             if constexpr (C::QHL) {
 #pragma unroll
               for (int j = 0; j < C::NT; ++j) {
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16(d, pl, vb[j][0], vb[j][1]);
+                float d[4];
+                mma_first<true>(d, pl, vb[j][0], vb[j][1]);
                 mma_f16(d, pa, vb[j][0], vb[j][1]);
 #pragma unroll
                 for (int f = 0; f < 2 * RH; ++f) o[j][f] += d[f];
