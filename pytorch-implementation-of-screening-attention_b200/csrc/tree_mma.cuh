@@ -446,6 +446,19 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
       }
     };
 
+    // --- the first stages, under way while the queries are brought in ------------
+    auto start = [&]() -> long long {
+      // the group's stage number `turn` sits in ring slot turn % S
+      long long rows[S];
+#pragma unroll
+      for (int i = 0; i < S; ++i) rows[i] = key_row(s0 + wk + i * C::WK);
+#pragma unroll
+      for (int i = 0; i < S - 1; ++i) load_stage(i, i, rows[i], false);
+      if (C::MG > 1 && mg == (S - 1) % C::MG) make_plan(S - 1, rows[S - 1]);
+      return rows[S - 1];
+    };
+    long long next = rg.any ? start() : -1;
+
     // --- queries: fragments, per-row factors ------------------------------------
     uint32_t qa[C::KS][4];
     uint32_t ql[C::QHL ? C::KS : 1][4];
@@ -550,14 +563,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
 #pragma unroll
         for (int f = 0; f < 4; ++f) o[j][f] = 0.f;
       if (rg.any) {
-        // the group's stage number `turn` sits in ring slot turn % S
-        long long rows[S - 1], next;
-#pragma unroll
-        for (int i = 0; i < S - 1; ++i) rows[i] = key_row(s0 + wk + i * C::WK);
-        next = key_row(s0 + wk + (S - 1) * C::WK);
-#pragma unroll
-        for (int i = 0; i < S - 1; ++i) load_stage(i, i, rows[i], false);
-        if (C::MG > 1 && mg == (S - 1) % C::MG) make_plan(S - 1, next);
+        if (pass == 1) next = start();
         int slot = 0, fill = S - 1, buf = 0;
         if constexpr (C::CONV) {
           cp_async_wait<S - 2>();
