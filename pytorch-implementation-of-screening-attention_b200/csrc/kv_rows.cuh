@@ -17,6 +17,19 @@ __device__ __forceinline__ long long paged_row(const screen_kv_cache& c, int b, 
   return ((long long)page * H + h) * c.page_size + (pos - blk * c.page_size);
 }
 
+// The same from a sequence's table row, in 32 bits; a shift where the page size
+// is a power of two.
+__device__ __forceinline__ long long table_row(const screen_kv_cache& c, const int* table, int H,
+                                               int h, long long pos) {
+  if (pos < 0 || pos > 0x7fffffff) return -1;
+  const unsigned p = (unsigned)pos, ps = (unsigned)c.page_size;
+  const unsigned blk = (ps & (ps - 1)) == 0 ? p >> (31 - __clz(ps)) : p / ps;
+  if (blk >= (unsigned)c.max_blocks) return -1;
+  const int page = table[blk];
+  if (page < 0 || page >= c.num_pages) return -1;
+  return ((long long)page * H + h) * ps + (p - blk * ps);
+}
+
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, float (&x)[4]);
 template <>
@@ -31,8 +44,19 @@ __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, flo
   x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
 
-// The int8 form of a raw row x held by a group of G lanes, E elements a lane (E a
-// multiple of 4), packed four to a word:
+template <typename T>
+__device__ __forceinline__ void load8f(const T* p, float (&x)[8]) {
+  float a[4], b[4];
+  load4(p, a);
+  load4(p + 4, b);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] = a[e];
+    x[4 + e] = b[e];
+  }
+}
+
+// The int8 form of a raw row x:
 //   m = round_half_even(127 x / max|x|),  scale = 1 / max(|m|, 127 eps / max|x|),
 // so scale * m is the unit form of the rounded raw row.  The integers do not
 // depend on any order of summation: max|x| is exact, and |m|^2 <= 128 * 127^2 is
@@ -41,7 +65,79 @@ __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, flo
 // remainder step), which no half can cross; for fp32 a quotient so near a half
 // that 32 bits cannot tell (127 * 2^-23 at most; one in 16,000) is decided by an
 // exact comparison in 64 bits.  A row with an infinity or NaN becomes m = 0, scale
-// NaN.  All 32 lanes of the warp must call it; x is used up.
+// NaN.
+struct Int8Scale {
+  float up, am, inv;     // x is scaled by up (0: a row of zeros); am = max|up x|
+};
+// of a row whose largest magnitude has the bits `top`
+__device__ __forceinline__ Int8Scale int8_scale(uint32_t top) {
+  const bool finite = top < 0x7f800000u;
+  const float amax = __uint_as_float(top);
+  Int8Scale s{1.0f, amax, 0.f};
+  if (!(amax > 1.0e-30f && amax < 1.0e30f)) {
+    // outside the reciprocal's range: scaled by a power of two; a row of zeros
+    // or with a non-finite value becomes zeros
+    s.up = finite && top ? (amax < 1.0f ? 0x1p100f : 0x1p-100f) : 0.f;
+    s.am = s.up != 0.f ? amax * s.up : 1.0f;
+  }
+  s.inv = 1.0f / s.am;
+  return s;
+}
+// E elements as int8, four to a word, and the sum of their squares added to ss.
+template <int E, bool BF>
+__device__ __forceinline__ void int8_pack(float (&x)[E], const Int8Scale& s, uint32_t (&m)[E / 4], int& ss) {
+  if (s.up != 1.0f) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = s.up != 0.f ? x[e] * s.up : 0.f;
+  }
+  const float magic = 12582912.0f;   // 1.5 * 2^23: rounds to an integer in the low byte
+  float f[E];
+  if constexpr (BF) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float d = 127.0f * x[e], q = d * s.inv;
+      f[e] = fmaf(fmaf(-q, s.am, d), s.inv, q) + magic;
+    }
+  } else {
+    bool near = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float t = 127.0f * x[e] * s.inv;
+      f[e] = t + magic;
+      near = near || fabsf(t - (f[e] - magic)) > 0.5f - 0x1p-15f;
+    }
+    if (near) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float t = fabsf(127.0f * x[e] * s.inv), k = floorf(t);
+        if (fabsf(t - k - 0.5f) < 0x1p-15f) {
+          const double num = 127.0 * (double)fabsf(x[e]), half = ((double)k + 0.5) * (double)s.am;
+          const bool odd = (int)k & 1;
+          f[e] = copysignf(num > half || (num == half && odd) ? k + 1.0f : k, x[e]) + magic;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < E / 4; ++w) {
+    const uint32_t a = __float_as_uint(f[4 * w]), b = __float_as_uint(f[4 * w + 1]);
+    const uint32_t c = __float_as_uint(f[4 * w + 2]), d = __float_as_uint(f[4 * w + 3]);
+    m[w] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+    ss = __dp4a((int)m[w], (int)m[w], ss);
+  }
+}
+// The stored scale of a row, ss = |m|^2.
+__device__ __forceinline__ float int8_stored_scale(uint32_t top, int ss, float eps) {
+  // 1 / |m| by one Newton step from the approximate reciprocal root
+  const float amax = __uint_as_float(top), n2 = (float)ss, y = rsqrtf(n2);
+  float scale = fmaf(0.5f * y, fmaf(-n2 * y, y, 1.0f), y);
+  // |m| >= 127: only a row below eps can meet the other bound, 1 / max(a, b) as
+  // min(1 / a, 1 / b)
+  if (!(amax >= eps)) scale = top ? fminf(scale, amax / (127.0f * eps)) : 0.f;
+  return top < 0x7f800000u ? scale : __uint_as_float(0x7fc00000u);
+}
+// A row held by a group of G lanes, E elements a lane.  All 32 lanes of the warp
+// must call it; x is used up.
 template <int G, int E, bool BF>
 __device__ __forceinline__ void int8_row(float (&x)[E], float eps, uint32_t (&m)[E / 4],
                                          float& scale) {
@@ -50,92 +146,11 @@ __device__ __forceinline__ void int8_row(float (&x)[E], float eps, uint32_t (&m)
   for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o, G));
-  const bool finite = top < 0x7f800000u;
-  const float amax = __uint_as_float(top);
-  float am = amax;
-  if (!(amax > 1.0e-30f && amax < 1.0e30f)) {
-    // outside the reciprocal's range: scaled by a power of two; a row of zeros
-    // or with a non-finite value becomes zeros
-    const float up = finite && top ? (amax < 1.0f ? 0x1p100f : 0x1p-100f) : 0.f;
-    am = up != 0.f ? amax * up : 1.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = up != 0.f ? x[e] * up : 0.f;
-  }
-  const float inv = 1.0f / am;
-  const float magic = 12582912.0f;   // 1.5 * 2^23: rounds to an integer in the low byte
-  float f[E];
-  if constexpr (BF) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float d = 127.0f * x[e], q = d * inv;
-      f[e] = fmaf(fmaf(-q, am, d), inv, q) + magic;
-    }
-  } else {
-    bool near = false;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float t = 127.0f * x[e] * inv;
-      f[e] = t + magic;
-      near = near || fabsf(t - (f[e] - magic)) > 0.5f - 0x1p-15f;
-    }
-    if (near) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float t = fabsf(127.0f * x[e] * inv), k = floorf(t);
-        if (fabsf(t - k - 0.5f) < 0x1p-15f) {
-          const double num = 127.0 * (double)fabsf(x[e]), half = ((double)k + 0.5) * (double)am;
-          const bool odd = (int)k & 1;
-          f[e] = copysignf(num > half || (num == half && odd) ? k + 1.0f : k, x[e]) + magic;
-        }
-      }
-    }
-  }
   int ss = 0;
-#pragma unroll
-  for (int w = 0; w < E / 4; ++w) {
-    const uint32_t a = __float_as_uint(f[4 * w]), b = __float_as_uint(f[4 * w + 1]);
-    const uint32_t c = __float_as_uint(f[4 * w + 2]), d = __float_as_uint(f[4 * w + 3]);
-    m[w] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-    ss = __dp4a((int)m[w], (int)m[w], ss);
-  }
+  int8_pack<E, BF>(x, int8_scale(top), m, ss);
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
-  // 1 / |m| by one Newton step from the approximate reciprocal root
-  const float n2 = (float)ss, y = rsqrtf(n2);
-  scale = fmaf(0.5f * y, fmaf(-n2 * y, y, 1.0f), y);
-  // |m| >= 127: only a row below eps can meet the other bound, 1 / max(a, b) as
-  // min(1 / a, 1 / b)
-  if (!(amax >= eps)) scale = top ? fminf(scale, amax / (127.0f * eps)) : 0.f;
-  if (!finite) scale = __uint_as_float(0x7fc00000u);
-}
-
-// Write the cache form of one raw row (G = D / 4 lanes, 4 elements a lane) at
-// row index `row` (< 0: nothing is written; the lanes still take part in the
-// shuffles).  T: the raw row's type.  E = signed char: int8 row and scale; else
-// the unit row in E with
-// the arithmetic of kv_append_kernel.
-template <typename E, typename T, int D>
-__device__ __forceinline__ void write_cache_row(float (&x)[4], float eps, int gl,
-                                                long long row, E* pages, float* scales) {
-  constexpr int G = D / 4;
-  if constexpr (sizeof(E) == 1) {
-    uint32_t m[1];
-    float sc;
-    int8_row<G, 4, sizeof(T) == 2>(x, eps, m, sc);
-    if (row >= 0) {
-      *reinterpret_cast<uint32_t*>(pages + row * D + gl * 4) = m[0];
-      if (gl == 0) scales[row] = sc;
-    }
-  } else {
-    float ss = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
-    const float nrm = fmaxf(sqrtf(ss), eps);
-    if (row >= 0) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pages[row * D + gl * 4 + e] = from_f<E>(x[e] / nrm);
-    }
-  }
+  scale = int8_stored_scale(top, ss, eps);
 }
 
 }  // namespace screen

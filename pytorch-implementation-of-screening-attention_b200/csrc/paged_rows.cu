@@ -33,18 +33,6 @@ __device__ __forceinline__ RowBlock row_block(int B, int H, int n, int tokens) {
   r.rows = min(tokens, n - r.n0) * H;
   return r;
 }
-// paged_row() for a sequence's table row
-__device__ __forceinline__ long long table_row(const screen_kv_cache& c, const int* table, int H,
-                                               int h, long long pos) {
-  if (pos < 0 || pos > 0x7fffffff) return -1;
-  const unsigned p = (unsigned)pos, ps = (unsigned)c.page_size;
-  const unsigned blk = (ps & (ps - 1)) == 0 ? p >> (31 - __clz(ps)) : p / ps;
-  if (blk >= (unsigned)c.max_blocks) return -1;
-  const int page = table[blk];
-  if (page < 0 || page >= c.num_pages) return -1;
-  return ((long long)page * H + h) * ps + (p - blk * ps);
-}
-
 // ---------------------------------------------------------------------------
 // Append to int8 pages.  Bound by HBM: D * sizeof(T) bytes in, D + 4 out per
 // row.

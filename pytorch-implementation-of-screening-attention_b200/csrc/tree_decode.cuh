@@ -213,30 +213,111 @@ __device__ __forceinline__ void tree_nodes(const screen_tree_args& a, int b, Nod
   __syncwarp();
 }
 
-// Rows of the nodes whose slots lie in the tiles [c0, c1] written to the pages.
+// Rows of the nodes whose slots lie in the tiles [c0, c1] written to the pages: a
+// thread per 8 elements, up to four of them in flight, the parts of a row meeting
+// in `scratch` (kAppendScratch bytes of shared memory).  A whole row per lane group
+// or per thread took up to 20 us for a tree of 64.  fp32 / bf16 pages: the sums of
+// kv_append_kernel (four elements, then halves of the D / 4 partial sums).
+constexpr int kAppendChunks = 4 * kThreads;
+constexpr int kAppendScratch = kAppendChunks * 8;
 template <typename E, typename TA, int D>
 __device__ __forceinline__ void append_rows(const screen_tree_args& a, const Nodes& nodes, int b,
-                                            int h, long long lens, int c0, int c1) {
-  constexpr int G = D / 4, RPI = kThreads / G;
-  const int tid = threadIdx.x, gl = tid % G;
+                                            int h, long long lens, int c0, int c1, void* scratch) {
+  constexpr int N = 8, C = D / N, U = kAppendChunks / kThreads;
+  constexpr bool kI8 = sizeof(E) == 1;
+  float2* part = reinterpret_cast<float2*>(scratch);
   long long lo = (long long)c0 * kTile - lens, hi = (long long)(c1 + 1) * kTile - 1 - lens;
   if (lo < 0) lo = 0;
   if (hi > a.n - 1) hi = a.n - 1;
-  const int cnt = hi >= lo ? (int)(hi - lo + 1) : 0;
-  for (int base = 0; base < 2 * cnt; base += RPI) {   // uniform over the CTA
-    const int u = base + tid / G;
-    const bool in = u < 2 * cnt;
-    const bool isv = in && u >= cnt;
-    const int i = in ? (int)lo + (isv ? u - cnt : u) : 0;
-    const bool take = in && nodes.line[i] != 0;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (take)
-      load4(reinterpret_cast<const TA*>(isv ? a.v : a.k) + (long long)b * (isv ? a.v_sb : a.k_sb) +
-                (long long)i * (isv ? a.v_st : a.k_st) + (long long)h * D + gl * 4, x);
-    const long long row = take ? paged_row(a.cache, b, a.H, h, lens + i) : -1;
-    write_cache_row<E, TA, D>(x, a.eps, gl, row,
-                          reinterpret_cast<E*>(isv ? a.cache.v_pages : a.cache.k_pages),
-                          isv ? a.v_scales : a.k_scales);
+  const int cnt = hi >= lo ? (int)(hi - lo + 1) : 0, chunks = 2 * cnt * C;
+  const int* table = a.cache.block_table + (long long)b * a.cache.max_blocks;
+#pragma unroll 1
+  for (int base = 0; base < chunks; base += kAppendChunks) {   // whole rows: C divides it
+    float x[U][N];
+    long long row[U];
+    // chunk u of the batch: row (base + u) / C (K rows, then V rows), element 8 (u % C)
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int u = base + k * kThreads + threadIdx.x, r = u / C;
+      const bool isv = r >= cnt;
+      const int i = (int)lo + (isv ? r - cnt : r);
+      row[k] = -1;
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[k][e] = 0.f;
+      if (u < chunks && nodes.line[i]) {
+        load8f(reinterpret_cast<const TA*>(isv ? a.v : a.k) + (long long)b * (isv ? a.v_sb : a.k_sb) +
+                   (long long)i * (isv ? a.v_st : a.k_st) + (long long)h * D + u % C * N, x[k]);
+        row[k] = table_row(a.cache, table, a.H, h, lens + i);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      float2 p;
+      if constexpr (kI8) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
+        p = make_float2(__uint_as_float(top), 0.f);
+      } else {
+        const float* v = x[k];
+        p.x = v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3];
+        p.y = v[4] * v[4] + v[5] * v[5] + v[6] * v[6] + v[7] * v[7];
+      }
+      part[k * kThreads + threadIdx.x] = p;
+    }
+    __syncthreads();
+    uint32_t tops[U];
+    int ss[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int u = k * kThreads + threadIdx.x, c = u % C;
+      const float2* mine = part + (u - c);
+      E* dst = reinterpret_cast<E*>((base + u) / C >= cnt ? a.cache.v_pages : a.cache.k_pages) +
+               row[k] * D + c * N;
+      if constexpr (kI8) {
+        tops[k] = 0;
+#pragma unroll
+        for (int j = 0; j < C; ++j) tops[k] = max(tops[k], __float_as_uint(mine[j].x));
+        uint32_t m[2];
+        ss[k] = 0;
+        int8_pack<N, sizeof(TA) == 2>(x[k], int8_scale(tops[k]), m, ss[k]);
+        if (row[k] >= 0) *reinterpret_cast<uint2*>(dst) = make_uint2(m[0], m[1]);
+      } else {
+        float p[2 * C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          p[2 * j] = mine[j].x;
+          p[2 * j + 1] = mine[j].y;
+        }
+#pragma unroll
+        for (int o = C; o > 0; o >>= 1)
+#pragma unroll
+          for (int j = 0; j < o; ++j) p[j] += p[j + o];
+        const float nrm = fmaxf(sqrtf(p[0]), a.eps);
+        if (row[k] >= 0) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) dst[e] = from_f<E>(x[k][e] / nrm);
+        }
+      }
+    }
+    __syncthreads();
+    if constexpr (kI8) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) part[k * kThreads + threadIdx.x].y = __int_as_float(ss[k]);
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int u = k * kThreads + threadIdx.x;
+        if (u % C == 0 && row[k] >= 0) {
+          int sum = 0;
+#pragma unroll
+          for (int j = 0; j < C; ++j) sum += __float_as_int(part[u + j].y);
+          ((base + u) / C >= cnt ? a.v_scales : a.k_scales)[row[k]] =
+              int8_stored_scale(tops[k], sum, a.eps);
+        }
+      }
+      __syncthreads();
+    }
   }
   __syncthreads();
 }

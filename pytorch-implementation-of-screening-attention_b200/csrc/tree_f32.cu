@@ -20,6 +20,7 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(TreeParams p, float*
   float* kt = qs + (size_t)p.a.n * D;              // [32][LD]
   float* vt = kt + kKeys * LD;
   float* al = vt + kKeys * LD;                     // [n][33]
+  static_assert(2 * kKeys * LD * 4 >= kAppendScratch, "append_rows works in the key tiles");
   __shared__ Nodes nodes;
   __shared__ int c_s[kKeys];
   __shared__ long long row_s[kKeys];
@@ -42,7 +43,7 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(TreeParams p, float*
   __syncthreads();   // the previous piece is done with the shared arrays
   if (warp == 0) tree_nodes(a, b, nodes, lane);
   __syncthreads();
-  if (rg.any && a.k) append_rows<float, float, D>(a, nodes, b, h, lens, c0, c1);
+  if (rg.any && a.k) append_rows<float, float, D>(a, nodes, b, h, lens, c0, c1, kt);
   for (int i = warp; i < n; i += 4) {
     const float* q = reinterpret_cast<const float*>(a.q) + (long long)b * a.q_sb +
                      (long long)i * a.q_st + (long long)h * D;

@@ -95,6 +95,7 @@ struct Cfg {
   static constexpr int GROUP_B = (PLAN_AT + PLAN_B + 15) / 16 * 16;
   static constexpr int RED_B = 4 * 16 * D_ * 4;       // the warps' sums at the end
   static constexpr int SMEM = WK * GROUP_B > RED_B ? WK * GROUP_B : RED_B;
+  static_assert(SMEM >= kAppendScratch, "append_rows works in it");
   // CTAs per SM the registers are cut to: what a thread holds of O and q decides
   static constexpr int HELD = D_ / 2 + D_ / 4 * (QHL ? 2 : 1);
   static constexpr int MINB = HELD <= 32 ? 4 : HELD <= 64 ? 3 : 2;
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
       __syncthreads();
       last_b = b;
     }
-    if (rg.any && a.k) append_rows<E, TA, D>(a, nodes, b, h, lens, c0, c1);
+    if (rg.any && a.k) append_rows<E, TA, D>(a, nodes, b, h, lens, c0, c1, dsm);
 
     // --- a stage: KT keys, their addresses and facts ---------------------------
     const int s0 = c0 * (kTile / KT), s1 = (c1 + 1) * (kTile / KT) - 1;
@@ -832,6 +833,22 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
           dst[o_col<C>(j, 2 * t + f)] = C::I8 ? o[j][2 * e + f] * 0x1p-20f : o[j][2 * e + f];
     }
     __syncthreads();
+    if (!whole) {
+      float4* dst = reinterpret_cast<float4*>(part + (size_t)(blockIdx.x + sh.seg) * a.n * D);
+      for (int u = tid; u < a.n * (D / 4); u += kThreads) {
+        float4 x = reinterpret_cast<const float4*>(red)[u];
+#pragma unroll
+        for (int k = 1; k < C::WK; ++k) {
+          const float4 y = reinterpret_cast<const float4*>(red + (size_t)k * ROWS * D)[u];
+          x.x += y.x;
+          x.y += y.y;
+          x.z += y.z;
+          x.w += y.w;
+        }
+        dst[u] = x;
+      }
+      continue;
+    }
     constexpr int PER = D < 32 ? 1 : D / 32;
     for (int i = warp; i < a.n; i += 4) {
       float x[PER];
@@ -842,14 +859,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
 #pragma unroll
           for (int k = 0; k < C::WK; ++k) x[e] += red[((size_t)k * ROWS + i) * D + lane + 32 * e];
       }
-      if (!whole) {
-        float* dst = part + ((size_t)(blockIdx.x + sh.seg) * a.n + i) * D;
-#pragma unroll
-        for (int e = 0; e < PER; ++e)
-          if (lane + 32 * e < D) dst[lane + 32 * e] = x[e];
-      } else {
-        store_row<TA, D>(a, b, i, h, lane, x, rg.any && nodes.line[i] != 0);
-      }
+      store_row<TA, D>(a, b, i, h, lane, x, rg.any && nodes.line[i] != 0);
     }
   }
 }
