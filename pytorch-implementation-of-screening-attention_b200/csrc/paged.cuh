@@ -10,6 +10,8 @@ void commit(const screen_commit_args& a, cudaStream_t s);
 
 // Positions are cut into tiles of kTreeTile keys.
 constexpr int kTreeTile = 64;
+// Segments (sequence, head) of a call whose tiles are shared out over CTAs.
+constexpr int kTreeMaxShared = 2048;
 struct TreeParams {
   screen_tree_args a;
   int lens_off;   // added to a.lens (decode: -1, the query is the newest cached token)

@@ -45,6 +45,13 @@ int tree_run(const screen_tree_args* a, int lens_off, cudaStream_t s) {
   if (!a->q || !a->lens || !a->r || !a->w || !a->y || (!a->k) != (!a->v))
     return SCREEN_ERR_INVALID_ARG;
   if ((long long)a->B * a->H > (1 << 28)) return SCREEN_ERR_UNSUPPORTED;
+  // more segments than the sharing out takes, or than CTAs: one CTA each
+  screen_tree_args one;
+  if (a->num_ctas > 1 && ((long long)a->B * a->H > kTreeMaxShared || (long long)a->B * a->H > a->num_ctas)) {
+    one = *a;
+    one.num_ctas = 1;
+    a = &one;
+  }
   int st = cache_ok(a->cache, a->cache_dtype, a->k_scales, a->v_scales);
   if (st) return st;
   if (!raw_ok(a->q, a->q_sb, a->q_st) || !al16(a->y)) return SCREEN_ERR_ALIGNMENT;
@@ -108,8 +115,7 @@ int screen_paged_read(const screen_paged_read_args* a, screen_stream_t stream) {
 
 size_t screen_tree_workspace_size(const screen_tree_args* a) {
   if (!a || tree_checks(a) || a->num_ctas == 1) return 0;
-  // a slot per (CTA, segment) pair along the tile list
-  return round_up((part_off(a) + ((size_t)a->B * a->H + a->num_ctas) * a->n * a->D) * sizeof(float));
+  return round_up((part_off(a) + (size_t)a->num_ctas * a->n * a->D) * sizeof(float));
 }
 
 int screen_tree_decode(const screen_tree_args* a, screen_stream_t stream) {

@@ -13,16 +13,17 @@
 // queries of a head.  The reads of the keys are what a pass cannot do without,
 // so the kernels are built around one pass over the pages.
 //
-// Sharing out the keys.  Positions are cut into 64-key tiles; the tiles of all
-// (sequence, head) segments, one after another, form one list that is cut into
-// equal runs, a CTA each.  Heads have windows of very different lengths (2 to
-// thousands of keys in one layer), so a fixed number of splits per head would
-// leave most CTAs idle while the widest head's work; the list needs no host
-// knowledge of lengths or windows.  A CTA that owns only a part of a segment
-// leaves its sum in workspace slot (CTA + segment), which no other pair shares
-// because both grow along the list, and tree_finish_kernel adds a segment's
-// slots in order.  With few tiles a segment goes to one CTA and no second launch
-// follows.
+// Sharing out the keys.  Heads have windows of very different lengths (2 to
+// thousands of keys in one layer), so a fixed number of splits per (sequence,
+// head) segment would leave most CTAs idle while the widest head's work.  Every
+// CTA reads all lengths and windows and finds the shortest run of 64-key tiles, L,
+// at which the segments, cut into ceil(tiles / L) equal runs each, fill the CTAs
+// that are resident at once; it then takes its own run.  No host knowledge of
+// lengths or windows is needed.  A run that is not a whole segment leaves its sum
+// in the workspace slot of its CTA, and tree_finish_kernel adds a segment's slots
+// in order.  (Cutting the list of all tiles into equal runs instead gave some
+// CTAs parts of two segments, and a part costs 6 us before its first tile.)  With
+// few tiles a segment goes to one CTA and no second launch follows.
 #pragma once
 #include "kv_rows.cuh"
 #include "paged.cuh"
@@ -59,111 +60,102 @@ __device__ __forceinline__ Range tree_range(const TreeParams& p, int b, int h) {
   return g;
 }
 
-// A CTA's run of the tile list, segment by segment.
-struct Share {
-  long long pos, end, start;   // next tile, end of the run, first tile of `seg`
-  long long total;
-  int ctas;                    // CTAs that have a run
-  int seg;
-};
-// Slots of the partial sums of each segment: CTAs first .. last, none if the
-// segment's rows were written by the CTA that owned all of it.
+// CTAs whose partial sums make up each segment: `count` from `first` on, 0 if the
+// CTA that owned all of it wrote the rows.
 struct SegSlots {
-  int first, last;
+  int first, count;
 };
-constexpr int kMinTiles = 4;   // a run is at least this long
-__device__ __forceinline__ long long share_begin(const Share& s, int cta) {
-  return s.total * cta / s.ctas;
-}
-// All threads of the CTA; false if it has nothing to do.
-__device__ __forceinline__ bool share_init(const TreeParams& p, Share& s) {
-  const int segs = p.a.B * p.a.H;
-  if (p.a.num_ctas == 1) {     // one CTA per segment
-    s.seg = blockIdx.x;
-    s.start = s.pos = 0;
-    s.ctas = 0;
-    return true;
-  }
-  __shared__ long long warp_s[kThreads / 32];
-  __shared__ long long start_s;
-  __shared__ int seg_s;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int each = (segs + kThreads - 1) / kThreads;
-  long long mine = 0;
-  for (int j = tid * each; j < (tid + 1) * each && j < segs; ++j)
-    mine += tree_range(p, j / p.a.H, j % p.a.H).nt;
-  long long inc = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += y;
-  }
-  if (lane == 31) warp_s[warp] = inc;
-  __syncthreads();
-  long long before = inc - mine;
-  s.total = 0;
-#pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) {
-    if (i < warp) before += warp_s[i];
-    s.total += warp_s[i];
-  }
-  const long long most = (s.total + kMinTiles - 1) / kMinTiles;
-  s.ctas = (long long)gridDim.x < most ? (int)gridDim.x : (int)most;
-  if ((int)blockIdx.x >= s.ctas) return false;
-  s.pos = share_begin(s, blockIdx.x);
-  s.end = share_begin(s, blockIdx.x + 1);
-  if (s.pos >= before && s.pos < before + mine) {   // this thread's segments hold it
-    int j = tid * each;
-    long long at = before;
-    while (true) {
-      const int nt = tree_range(p, j / p.a.H, j % p.a.H).nt;
-      if (s.pos < at + nt) break;
-      at += nt;
-      ++j;
-    }
-    seg_s = j;
-    start_s = at;
-  }
-  __syncthreads();
-  s.seg = seg_s;
-  s.start = start_s;
-  return true;
-}
-// Next piece: tiles [c0, c1] of segment s.seg.  False at the end of the run.
-__device__ __forceinline__ bool share_next(const TreeParams& p, Share& s, Range& g, int& c0,
-                                           int& c1, bool& whole, SegSlots* slots) {
-  if (s.ctas == 0) {
-    if (s.pos) return false;
-    g = tree_range(p, s.seg / p.a.H, s.seg % p.a.H);
+constexpr int kMinTiles = 4;         // a run is at least this long
+constexpr int kMaxShared = kTreeMaxShared;
+// This CTA's run: tiles [c0, c1] of segment seg.  False if there is none for it.
+// All threads of the CTA; `tiles` is kMaxShared ints of shared memory.
+__device__ __forceinline__ bool find_run(const TreeParams& p, int* tiles, SegSlots* slots, int& seg,
+                                         Range& g, int& c0, int& c1, bool& whole) {
+  const int segs = p.a.B * p.a.H, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (p.a.num_ctas == 1) {           // one CTA per segment
+    seg = blockIdx.x;
+    g = tree_range(p, seg / p.a.H, seg % p.a.H);
     c0 = g.t0;
     c1 = g.t0 + g.nt - 1;
     whole = true;
-    s.pos = 1;
     return true;
   }
-  if (s.pos >= s.end) return false;
-  if (s.pos >= s.start) {
-    g = tree_range(p, s.seg / p.a.H, s.seg % p.a.H);
-    while (s.pos >= s.start + g.nt) {   // the previous piece ended its segment
-      s.start += g.nt;
-      ++s.seg;
-      g = tree_range(p, s.seg / p.a.H, s.seg % p.a.H);
+  constexpr int NW = kThreads / 32;
+  __shared__ long long sum_s[NW];
+  __shared__ int run_s[2];
+  const int ctas = gridDim.x;
+  long long sum = 0;
+  for (int j = tid; j < segs; j += kThreads) {
+    const int nt = tree_range(p, j / p.a.H, j % p.a.H).nt;
+    tiles[j] = nt;
+    sum += nt;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sum_s[warp] = sum;
+  __syncthreads();
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) sum += sum_s[i];
+  // runs of L tiles: too many at lo - 1, few enough at hi; each warp counts one
+  // candidate a round
+  int lo = (int)((sum + ctas - 1) / ctas);
+  if (lo < kMinTiles) lo = kMinTiles;
+  int hi = ctas > segs ? (int)((sum + ctas - segs - 1) / (ctas - segs)) : 0x3fffffff;
+  if (hi < lo) hi = lo;
+  while (lo < hi) {
+    __syncthreads();
+    const int cand = lo + (int)((long long)(hi - lo) * warp / NW);
+    int runs = 0;
+    for (int j = lane; j < segs; j += 32) runs += (tiles[j] + cand - 1) / cand;
+    runs = __reduce_add_sync(0xffffffffu, runs);
+    if (lane == 0) sum_s[warp] = runs;
+    __syncthreads();
+    int l = lo, h = hi;
+#pragma unroll
+    for (int i = NW - 1; i >= 0; --i) {
+      const int c = lo + (int)((long long)(hi - lo) * i / NW);
+      if (sum_s[i] <= ctas) h = c;
+      else if (c + 1 > l) l = c + 1;
+    }
+    lo = l;
+    hi = h;
+    if (hi < lo) hi = lo;
+  }
+  __syncthreads();
+  if (warp == 0) {                   // the segment whose runs hold this CTA
+    int before = 0;
+    for (int j0 = 0; j0 < segs; j0 += 32) {
+      const int j = j0 + lane, n = j < segs ? (tiles[j] + hi - 1) / hi : 0;
+      int inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      const int mine = (int)blockIdx.x - (before + inc - n);
+      const unsigned who = __ballot_sync(0xffffffffu, mine >= 0 && mine < n);
+      if (who) {
+        if (lane == __ffs(who) - 1) {
+          run_s[0] = j;
+          run_s[1] = mine;
+        }
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+      if (j0 + 32 >= segs && lane == 0) run_s[0] = -1;
     }
   }
-  const long long stop = s.end < s.start + g.nt ? s.end : s.start + g.nt;
-  c0 = g.t0 + (int)(s.pos - s.start);
-  c1 = g.t0 + (int)(stop - s.start) - 1;
-  whole = s.pos == s.start && stop == s.start + g.nt;
-  if (s.pos == s.start && threadIdx.x == 0) {
-    SegSlots q{0, -1};
-    if (!whole) {
-      q.first = blockIdx.x;
-      // the last CTA whose run begins at or before the segment's last tile
-      q.last = (int)(((s.start + g.nt) * s.ctas - 1) / s.total);
-    }
-    slots[s.seg] = q;
-  }
-  s.pos = stop;
+  __syncthreads();
+  seg = run_s[0];
+  if (seg < 0) return false;
+  const int i = run_s[1], nt = tiles[seg], n = (nt + hi - 1) / hi;
+  __syncthreads();                   // `tiles` has been read
+  g = tree_range(p, seg / p.a.H, seg % p.a.H);
+  c0 = g.t0 + (int)((long long)nt * i / n);
+  c1 = g.t0 + (int)((long long)nt * (i + 1) / n) - 1;
+  whole = n == 1;
+  if (i == 0 && tid == 0) slots[seg] = SegSlots{(int)blockIdx.x, whole ? 0 : n};
   return true;
 }
 
@@ -341,12 +333,13 @@ __device__ __forceinline__ void store_row(const screen_tree_args& a, int b, int 
     if (lane + 32 * e < D) y[lane + 32 * e] = from_f<TA>(present ? o[e] * g : 0.f);
 }
 
-// One CTA per segment, or at most as many as are resident at once: a run for
-// each, all of one length.
+// One CTA per segment, or at most as many as are resident at once (a CTA per segment
+// at least).
 constexpr int kSMs = 148;
 inline dim3 tree_grid(const TreeParams& p, int per_sm) {
   if (p.a.num_ctas == 1) return dim3(p.a.B * p.a.H);
-  return dim3(p.a.num_ctas < kSMs * per_sm ? p.a.num_ctas : kSMs * per_sm);
+  const int segs = p.a.B * p.a.H, fit = kSMs * per_sm > segs ? kSMs * per_sm : segs;
+  return dim3(p.a.num_ctas < fit ? p.a.num_ctas : fit);
 }
 
 }  // namespace tree

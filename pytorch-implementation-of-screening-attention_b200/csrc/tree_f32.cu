@@ -31,16 +31,13 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(TreeParams p, float*
   const int n = a.n;
   SegSlots* slots = reinterpret_cast<SegSlots*>(ws);
   float* part = ws + p.part_off;
-  Share sh;
-  if (!share_init(p, sh)) return;
   Range rg;
-  int c0, c1;
+  int seg, c0, c1;
   bool whole;
-  while (share_next(p, sh, rg, c0, c1, whole, slots)) {
-  const int b = sh.seg / a.H, h = sh.seg % a.H;
+  if (!find_run(p, reinterpret_cast<int*>(fsm), slots, seg, rg, c0, c1, whole)) return;
+  const int b = seg / a.H, h = seg % a.H;
   const float w = a.w[h], r = a.r[h];
   const long long lens = rg.lens;
-  __syncthreads();   // the previous piece is done with the shared arrays
   if (warp == 0) tree_nodes(a, b, nodes, lane);
   __syncthreads();
   if (rg.any && a.k) append_rows<float, float, D>(a, nodes, b, h, lens, c0, c1, kt);
@@ -131,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(TreeParams p, float*
 #pragma unroll
     for (int e = 0; e < PER; ++e) x[e] = lane + 32 * e < D ? qs[i * D + lane + 32 * e] : 0.f;
     if (!whole) {
-      float* dst = part + ((size_t)(blockIdx.x + sh.seg) * n + i) * D;
+      float* dst = part + ((size_t)blockIdx.x * n + i) * D;
 #pragma unroll
       for (int e = 0; e < PER; ++e)
         if (lane + 32 * e < D) dst[lane + 32 * e] = x[e];
@@ -139,10 +136,9 @@ __global__ void __launch_bounds__(kThreads) tree_f32_kernel(TreeParams p, float*
       store_row<float, D>(a, b, i, h, lane, x, rg.any && nodes.line[i] != 0);
     }
   }
-  }
 }
 
-// Sum a segment's partials in the order of the list, TanhNorm, store; a warp per
+// Sum a segment's partials in the order of its runs, TanhNorm, store; a warp per
 // (segment, node).  The sum of an absent node is zero (nothing was seen).
 template <typename TA, int D>
 __global__ void __launch_bounds__(128) tree_finish_kernel(TreeParams p, const float* __restrict__ ws) {
@@ -155,13 +151,13 @@ __global__ void __launch_bounds__(128) tree_finish_kernel(TreeParams p, const fl
   if (row >= (long long)a.B * a.H * a.n) return;
   const int i = (int)(row % a.n), seg = (int)(row / a.n);
   const SegSlots q = reinterpret_cast<const SegSlots*>(ws)[seg];
-  if (q.last < q.first) return;   // written by the CTA that owned the segment
+  if (q.count == 0) return;   // written by the CTA that owned the segment
   float x[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) x[e] = 0.f;
-  const float* src = ws + p.part_off + ((size_t)seg * a.n + i) * D;
+  const float* src = ws + p.part_off + (size_t)i * D;
 #pragma unroll 4
-  for (int c = q.first; c <= q.last; ++c)
+  for (int c = q.first; c < q.first + q.count; ++c)
 #pragma unroll
     for (int e = 0; e < PER; ++e)
       if (lane + 32 * e < D) x[e] += src[(size_t)c * a.n * D + lane + 32 * e];
@@ -170,7 +166,8 @@ __global__ void __launch_bounds__(128) tree_finish_kernel(TreeParams p, const fl
 
 template <int D>
 void launch_f32(const TreeParams& p, float* part, cudaStream_t s) {
-  const size_t smem = ((size_t)p.a.n * D + 2 * kKeys * (D + 4) + (size_t)p.a.n * 33) * 4;
+  size_t smem = ((size_t)p.a.n * D + 2 * kKeys * (D + 4) + (size_t)p.a.n * 33) * 4;
+  if (smem < kMaxShared * 4) smem = kMaxShared * 4;   // find_run
   constexpr int kMost = (kMaxN * D + 2 * kKeys * (D + 4) + kMaxN * 33) * 4;
   if (ensure_smem_optin((const void*)tree_f32_kernel<D>, kMost) != cudaSuccess) return;
   launch_pdl(tree_f32_kernel<D>, tree_grid(p, 3), dim3(kThreads), smem, s, p, part);

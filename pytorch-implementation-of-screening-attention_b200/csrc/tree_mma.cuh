@@ -94,8 +94,9 @@ struct Cfg {
   static constexpr int PLAN_AT = RING_B + 4 * HALF_B;
   static constexpr int GROUP_B = (PLAN_AT + PLAN_B + 15) / 16 * 16;
   static constexpr int RED_B = 4 * 16 * D_ * 4;       // the warps' sums at the end
-  static constexpr int SMEM = WK * GROUP_B > RED_B ? WK * GROUP_B : RED_B;
-  static_assert(SMEM >= kAppendScratch, "append_rows works in it");
+  static constexpr int MAIN_B = WK * GROUP_B > RED_B ? WK * GROUP_B : RED_B;
+  static constexpr int SMEM = MAIN_B > kMaxShared * 4 ? MAIN_B : kMaxShared * 4;
+  static_assert(SMEM >= kAppendScratch && SMEM >= kMaxShared * 4, "append_rows and find_run work in it");
   // CTAs per SM the registers are cut to: what a thread holds of O and q decides
   static constexpr int HELD = D_ / 2 + D_ / 4 * (QHL ? 2 : 1);
   static constexpr int MINB = HELD <= 32 ? 4 : HELD <= 64 ? 3 : 2;
@@ -302,565 +303,558 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
   const int ps = a.cache.page_size;
   const int ps_shift = (ps & (ps - 1)) == 0 ? 31 - __clz(ps) : -1;
 
-  Share sh;
-  if (!share_init(p, sh)) return;
   Range rg;
-  int c0, c1, last_b = -1;
+  int seg, c0, c1;
   bool whole;
-  while (share_next(p, sh, rg, c0, c1, whole, slots)) {
-    const int b = sh.seg / a.H, h = sh.seg % a.H;
-    const float w = a.w[h], r = a.r[h];
-    const long long lens = rg.lens;
-    __syncthreads();   // the previous piece is done with the shared arrays
-    if (b != last_b) {
-      if (warp == 0) tree_nodes(a, b, nodes, lane);
-      __syncthreads();
-      last_b = b;
-    }
-    if (rg.any && a.k) append_rows<E, TA, D>(a, nodes, b, h, lens, c0, c1, dsm);
+  if (!find_run(p, reinterpret_cast<int*>(dsm), slots, seg, rg, c0, c1, whole)) return;
+  const int b = seg / a.H, h = seg % a.H;
+  const float w = a.w[h], r = a.r[h];
+  const long long lens = rg.lens;
+  if (warp == 0) tree_nodes(a, b, nodes, lane);
+  __syncthreads();
+  if (rg.any && a.k) append_rows<E, TA, D>(a, nodes, b, h, lens, c0, c1, dsm);
 
-    // --- a stage: KT keys, their addresses and facts ---------------------------
-    const int s0 = c0 * (kTile / KT), s1 = (c1 + 1) * (kTile / KT) - 1;
-    const int* table = a.cache.block_table + (long long)b * a.cache.max_blocks;
-    // row of this lane's key of stage x, -1 none
-    auto key_row = [&](int x) -> long long {
-      const long long pos = (long long)x * KT + lane;
-      if (lane >= KT || x > s1 || pos < rg.first || pos >= lens + a.n) return -1;
-      if (pos >= lens && !nodes.line[pos - lens]) return -1;
-      const unsigned q = (unsigned)pos;                // a table holds < 2^31 positions
-      const unsigned blk = ps_shift >= 0 ? q >> ps_shift : q / (unsigned)ps;
-      if (blk >= (unsigned)a.cache.max_blocks) return -1;
-      const int page = table[blk];
-      if (page < 0 || page >= a.cache.num_pages) return -1;
-      return ((long long)page * a.H + h) * ps + (q - blk * (unsigned)ps);
-    };
-    // In a group of several warps they take turns in looking a stage's rows up: its
-    // warp leaves them in a plan (rows, then the first row if all follow it, else
-    // -1) that the group reads after its next barrier.
-    auto plan = [&](int turn) {
-      return reinterpret_cast<long long*>(ring + C::PLAN_AT) + (turn & 1) * (KT + 1);
-    };
-    auto first_of_run = [&](long long row) -> long long {
-      const long long row0 = __shfl_sync(0xffffffffu, row, 0);
-      const bool run = __all_sync(0xffffffffu, lane >= KT || row == row0 + lane) && row0 >= 0;
-      return run ? row0 : -1;
-    };
-    auto make_plan = [&](int turn, long long row) {
-      const long long row0 = first_of_run(row);
-      long long* pl = plan(turn);
-      if (lane < KT) pl[lane] = row;
-      if (lane == 0) pl[KT] = row0;
-    };
-    // `row`: this lane's key, of the warp whose turn it is
-    auto load_stage = [&](int turn, int slot, long long row, bool planned) {
-      const int x = s0 + wk + turn * C::WK;
-      unsigned char* st = ring + (size_t)slot * C::STAGE_B;
-      if (x <= s1) {
-        const uint32_t sa = smem_u32(st);
-        const char* kp = reinterpret_cast<const char*>(a.cache.k_pages);
-        const char* vp = reinterpret_cast<const char*>(a.cache.v_pages);
-        const long long* pl = plan(turn);
-        const long long row0 = C::MG > 1 && planned ? pl[KT] : first_of_run(row);
-        if (row0 >= 0) {                               // all keys there, one after another
-          const long long off = row0 * C::RB + gt * 16;
+  // --- a stage: KT keys, their addresses and facts ---------------------------
+  const int s0 = c0 * (kTile / KT), s1 = (c1 + 1) * (kTile / KT) - 1;
+  const int* table = a.cache.block_table + (long long)b * a.cache.max_blocks;
+  // row of this lane's key of stage x, -1 none
+  auto key_row = [&](int x) -> long long {
+    const long long pos = (long long)x * KT + lane;
+    if (lane >= KT || x > s1 || pos < rg.first || pos >= lens + a.n) return -1;
+    if (pos >= lens && !nodes.line[pos - lens]) return -1;
+    const unsigned q = (unsigned)pos;                // a table holds < 2^31 positions
+    const unsigned blk = ps_shift >= 0 ? q >> ps_shift : q / (unsigned)ps;
+    if (blk >= (unsigned)a.cache.max_blocks) return -1;
+    const int page = table[blk];
+    if (page < 0 || page >= a.cache.num_pages) return -1;
+    return ((long long)page * a.H + h) * ps + (q - blk * (unsigned)ps);
+  };
+  // In a group of several warps they take turns in looking a stage's rows up: its
+  // warp leaves them in a plan (rows, then the first row if all follow it, else
+  // -1) that the group reads after its next barrier.
+  auto plan = [&](int turn) {
+    return reinterpret_cast<long long*>(ring + C::PLAN_AT) + (turn & 1) * (KT + 1);
+  };
+  auto first_of_run = [&](long long row) -> long long {
+    const long long row0 = __shfl_sync(0xffffffffu, row, 0);
+    const bool run = __all_sync(0xffffffffu, lane >= KT || row == row0 + lane) && row0 >= 0;
+    return run ? row0 : -1;
+  };
+  auto make_plan = [&](int turn, long long row) {
+    const long long row0 = first_of_run(row);
+    long long* pl = plan(turn);
+    if (lane < KT) pl[lane] = row;
+    if (lane == 0) pl[KT] = row0;
+  };
+  // `row`: this lane's key, of the warp whose turn it is
+  auto load_stage = [&](int turn, int slot, long long row, bool planned) {
+    const int x = s0 + wk + turn * C::WK;
+    unsigned char* st = ring + (size_t)slot * C::STAGE_B;
+    if (x <= s1) {
+      const uint32_t sa = smem_u32(st);
+      const char* kp = reinterpret_cast<const char*>(a.cache.k_pages);
+      const char* vp = reinterpret_cast<const char*>(a.cache.v_pages);
+      const long long* pl = plan(turn);
+      const long long row0 = C::MG > 1 && planned ? pl[KT] : first_of_run(row);
+      if (row0 >= 0) {                               // all keys there, one after another
+        const long long off = row0 * C::RB + gt * 16;
 #pragma unroll
-          for (int i = 0; i < (KT * C::CH + GT - 1) / GT; ++i) {
-            const int u = i * GT + gt;
-            if (KT * C::CH % GT == 0 || u < KT * C::CH) {
-              cp_async16(sa + k_off<C>(u / C::CH, u % C::CH), kp + off + i * GT * 16, true);
-              cp_async16(sa + C::TILE_B + v_off<C>(u / C::CH, u % C::CH), vp + off + i * GT * 16, true);
-            }
+        for (int i = 0; i < (KT * C::CH + GT - 1) / GT; ++i) {
+          const int u = i * GT + gt;
+          if (KT * C::CH % GT == 0 || u < KT * C::CH) {
+            cp_async16(sa + k_off<C>(u / C::CH, u % C::CH), kp + off + i * GT * 16, true);
+            cp_async16(sa + C::TILE_B + v_off<C>(u / C::CH, u % C::CH), vp + off + i * GT * 16, true);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < (KT * C::CH + GT - 1) / GT; ++i) {
+          const int u = i * GT + gt, k = u / C::CH;
+          long long at = __shfl_sync(0xffffffffu, row, k & (KT - 1));
+          if (C::MG > 1 && planned) at = pl[k & (KT - 1)];
+          if (k < KT) {
+            const long long off = (at < 0 ? 0 : at) * C::RB + u % C::CH * 16;
+            cp_async16(sa + k_off<C>(k, u % C::CH), kp + off, at >= 0);
+            cp_async16(sa + C::TILE_B + v_off<C>(k, u % C::CH), vp + off, at >= 0);
+          }
+        }
+      }
+      if (mg == turn % C::MG) {
+        // this lane's key, stored at its score column
+        const int k = lane & (KT - 1);
+        const int col = (k & ~7) | key_of<C>(k & 7); // key_of is its own inverse
+        float* cs = reinterpret_cast<float*>(st + 2 * C::TILE_B);
+        if constexpr (C::I8) {
+          // KT = 16: lanes 16-31 fetch the V scales
+          const long long at = KT == 32 ? row : __shfl_sync(0xffffffffu, row, k);
+          const long long off = at < 0 ? 0 : at;
+          if (KT == 32 || lane < KT)
+            cp_async4(smem_u32(cs + 2 * KT + col), a.k_scales + off, at >= 0);
+          if (KT == 32 || lane >= KT)
+            cp_async4(smem_u32(cs + 3 * KT + col), a.v_scales + off, at >= 0);
+        }
+        const long long pos = (long long)x * KT + lane;
+        int c = kNoKey;
+        if (row >= 0) c = pos < lens ? (int)(pos - lens) : nodes.depth[pos - lens];
+        // a score needs its own window / ancestor test next to the window's
+        // old end, in the nodes' own slots, and where a key is missing
+        const bool e = lane < KT && (c == kNoKey || pos >= lens || pos < lens - rg.dmax + kMaxN);
+        const unsigned edge = __ballot_sync(0xffffffffu, e);
+        if (lane < KT) {
+          float sn = 0.f, cn = 0.f;
+          if (c != kNoKey) sincospif((float)c / w, &sn, &cn);
+          cs[col] = cn;
+          cs[KT + col] = sn;
+          reinterpret_cast<int*>(cs)[(C::I8 ? 4 : 2) * KT + col] = c;
+        }
+        if (lane == 0) reinterpret_cast<int*>(cs)[(C::I8 ? 5 : 3) * KT] = edge != 0;
+      }
+    }
+    cp_async_commit();
+  };
+  // CONV: a landed int8 stage as fp16 tiles for ldmatrix
+  auto widen_stage = [&](int slot, int buf) {
+    const unsigned char* kt = ring + (size_t)slot * C::STAGE_B;
+    unsigned char* kh = half + (size_t)buf * 2 * C::HALF_B;
+#pragma unroll
+    for (int i = 0; i < (KT * C::CH + GT - 1) / GT; ++i) {
+      const int u = i * GT + gt;
+      if (KT * C::CH % GT == 0 || u < KT * C::CH) {
+        const int k = u / C::CH, c = u % C::CH;
+        const uint4 x = *reinterpret_cast<const uint4*>(kt + k_off<C>(k, c));
+        const uint4 y = *reinterpret_cast<const uint4*>(kt + C::TILE_B + v_off<C>(k, c));
+        uint4 x0, x1, y0, y1;
+        widen16(x, x0, x1);
+        widen16(y, y0, y1);
+        *reinterpret_cast<uint4*>(kh + off16<C::CH16>(k, 2 * c)) = x0;
+        *reinterpret_cast<uint4*>(kh + off16<C::CH16>(k, 2 * c + 1)) = x1;
+        *reinterpret_cast<uint4*>(kh + C::HALF_B + off16<C::CH16>(k, 2 * c)) = y0;
+        *reinterpret_cast<uint4*>(kh + C::HALF_B + off16<C::CH16>(k, 2 * c + 1)) = y1;
+      }
+    }
+    // the mask's factors with the V row's scale in them, once for all warps
+    if (gt < KT) {
+      float* cs = reinterpret_cast<float*>(ring + (size_t)slot * C::STAGE_B + 2 * C::TILE_B) + gt;
+      const float vs = cs[3 * KT];
+      cs[0] *= vs;
+      cs[KT] *= vs;
+      cs[3 * KT] = vs * 0x1p19f;
+    }
+  };
+
+  // --- the first stages, under way while the queries are brought in ------------
+  auto start = [&]() -> long long {
+    // the group's stage number `turn` sits in ring slot turn % S
+    long long rows[S];
+#pragma unroll
+    for (int i = 0; i < S; ++i) rows[i] = key_row(s0 + wk + i * C::WK);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) load_stage(i, i, rows[i], false);
+    if (C::MG > 1 && mg == (S - 1) % C::MG) make_plan(S - 1, rows[S - 1]);
+    return rows[S - 1];
+  };
+  long long next = rg.any ? start() : -1;
+
+  // --- queries: fragments, per-row factors ------------------------------------
+  uint32_t qa[C::KS][4];
+  uint32_t ql[C::QHL ? C::KS : 1][4];
+  float rq[RH], ci[RH], si[RH];
+  int dep[RH];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (e >= RH) {
+#pragma unroll
+      for (int s = 0; s < C::KS; ++s) {
+        qa[s][1] = qa[s][3] = 0u;
+        if constexpr (C::QHL) ql[s][1] = ql[s][3] = 0u;
+      }
+      continue;
+    }
+    const int i = mg * 16 + g + 8 * e;
+    const bool in = i < a.n && rg.any;
+    const TA* q = reinterpret_cast<const TA*>(a.q) + (long long)b * a.q_sb + (long long)i * a.q_st +
+                  (long long)h * D;
+    float x[C::KS][4];
+    float ss = 0.f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < C::KS; ++s)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        x[s][2 * f] = x[s][2 * f + 1] = 0.f;
+        if (in) {
+          if constexpr (sizeof(TA) == 2) {
+            const float2 v = unpack_bf16(*reinterpret_cast<const uint32_t*>(q + d_of<C>(t, s, f)));
+            x[s][2 * f] = v.x;
+            x[s][2 * f + 1] = v.y;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(q + d_of<C>(t, s, f));
+            x[s][2 * f] = v.x;
+            x[s][2 * f + 1] = v.y;
+          }
+        }
+      }
+#pragma unroll
+    for (int s = 0; s < C::KS; ++s)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        ss = fmaf(x[s][f], x[s][f], ss);
+        top = max(top, __float_as_uint(x[s][f]) & 0x7fffffffu);
+      }
+    ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+    ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+    float scale = 1.f;
+    if constexpr (C::I8) {
+      // bring the row's largest element into [1, 2): the bf16 row is then
+      // exact in fp16 (elements under 2^-16 of the largest round at 2^-25
+      // of it), an fp32 row is held as hi + lo halves to 2^-25
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int ex = (int)(top >> 23);
+      ex = ex < 1 ? 1 : ex > 253 ? 253 : ex;
+      const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
+      scale = __uint_as_float((uint32_t)ex << 23);
+#pragma unroll
+      for (int s = 0; s < C::KS; ++s)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) x[s][f] *= down;
+    }
+#pragma unroll
+    for (int s = 0; s < C::KS; ++s)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        if constexpr (C::I8) {
+          qa[s][2 * f + e] = pack_f16(x[s][2 * f], x[s][2 * f + 1]);
+          if constexpr (C::QHL) {
+            const float2 u = __half22float2(*reinterpret_cast<__half2*>(&qa[s][2 * f + e]));
+            ql[s][2 * f + e] = pack_f16(x[s][2 * f] - u.x, x[s][2 * f + 1] - u.y);
           }
         } else {
+          qa[s][2 * f + e] = pack_bf16(x[s][2 * f], x[s][2 * f + 1]);
+        }
+      }
+    // S = q.k scale / max(|q|, eps), times r; scale first: 2^ex / |q| <= 1
+    rq[e] = r * (scale / fmaxf(sqrtf(ss), a.eps));
+    const bool live = in && nodes.line[i] != 0;
+    dep[e] = live ? nodes.depth[i] : 0;
+    float sn, cn;
+    sincospif((float)dep[e] / w, &sn, &cn);
+    // int8: alpha carries the V row's scale <= 1 / 127; 2^20 keeps it normal
+    // in fp16 down to alpha = 2^-23
+    ci[e] = (C::I8 ? 0x1p19f : 0.5f) * cn;
+    si[e] = (C::I8 ? 0x1p19f : 0.5f) * sn;
+    if (!live) rq[e] = __uint_as_float(0x7fc00000u);  // t = NaN: sees nothing
+  }
+  const float2 one_r = both(1.0f - r);
+
+  float o[C::NT][4];
+  // pass 0 takes every V row and scale as finite.  A non-finite one times
+  // alpha = 0 would spoil queries that do not see it: if any sum comes out
+  // non-finite, pass 1 repeats the run with such rows left out of the product
+  // and put back as NaN for the queries that see them.
 #pragma unroll 1
-          for (int i = 0; i < (KT * C::CH + GT - 1) / GT; ++i) {
-            const int u = i * GT + gt, k = u / C::CH;
-            long long at = __shfl_sync(0xffffffffu, row, k & (KT - 1));
-            if (C::MG > 1 && planned) at = pl[k & (KT - 1)];
-            if (k < KT) {
-              const long long off = (at < 0 ? 0 : at) * C::RB + u % C::CH * 16;
-              cp_async16(sa + k_off<C>(k, u % C::CH), kp + off, at >= 0);
-              cp_async16(sa + C::TILE_B + v_off<C>(k, u % C::CH), vp + off, at >= 0);
-            }
-          }
-        }
-        if (mg == turn % C::MG) {
-          // this lane's key, stored at its score column
-          const int k = lane & (KT - 1);
-          const int col = (k & ~7) | key_of<C>(k & 7); // key_of is its own inverse
-          float* cs = reinterpret_cast<float*>(st + 2 * C::TILE_B);
-          if constexpr (C::I8) {
-            // KT = 16: lanes 16-31 fetch the V scales
-            const long long at = KT == 32 ? row : __shfl_sync(0xffffffffu, row, k);
-            const long long off = at < 0 ? 0 : at;
-            if (KT == 32 || lane < KT)
-              cp_async4(smem_u32(cs + 2 * KT + col), a.k_scales + off, at >= 0);
-            if (KT == 32 || lane >= KT)
-              cp_async4(smem_u32(cs + 3 * KT + col), a.v_scales + off, at >= 0);
-          }
-          const long long pos = (long long)x * KT + lane;
-          int c = kNoKey;
-          if (row >= 0) c = pos < lens ? (int)(pos - lens) : nodes.depth[pos - lens];
-          // a score needs its own window / ancestor test next to the window's
-          // old end, in the nodes' own slots, and where a key is missing
-          const bool e = lane < KT && (c == kNoKey || pos >= lens || pos < lens - rg.dmax + kMaxN);
-          const unsigned edge = __ballot_sync(0xffffffffu, e);
-          if (lane < KT) {
-            float sn = 0.f, cn = 0.f;
-            if (c != kNoKey) sincospif((float)c / w, &sn, &cn);
-            cs[col] = cn;
-            cs[KT + col] = sn;
-            reinterpret_cast<int*>(cs)[(C::I8 ? 4 : 2) * KT + col] = c;
-          }
-          if (lane == 0) reinterpret_cast<int*>(cs)[(C::I8 ? 5 : 3) * KT] = edge != 0;
-        }
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+    for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) o[j][f] = 0.f;
+    if (rg.any) {
+      if (pass == 1) next = start();
+      int slot = 0, fill = S - 1, buf = 0;
+      if constexpr (C::CONV) {
+        cp_async_wait<S - 2>();
+        group_sync();
+        if (s0 + wk <= s1) widen_stage(0, 0);
       }
-      cp_async_commit();
-    };
-    // CONV: a landed int8 stage as fp16 tiles for ldmatrix
-    auto widen_stage = [&](int slot, int buf) {
-      const unsigned char* kt = ring + (size_t)slot * C::STAGE_B;
-      unsigned char* kh = half + (size_t)buf * 2 * C::HALF_B;
-#pragma unroll
-      for (int i = 0; i < (KT * C::CH + GT - 1) / GT; ++i) {
-        const int u = i * GT + gt;
-        if (KT * C::CH % GT == 0 || u < KT * C::CH) {
-          const int k = u / C::CH, c = u % C::CH;
-          const uint4 x = *reinterpret_cast<const uint4*>(kt + k_off<C>(k, c));
-          const uint4 y = *reinterpret_cast<const uint4*>(kt + C::TILE_B + v_off<C>(k, c));
-          uint4 x0, x1, y0, y1;
-          widen16(x, x0, x1);
-          widen16(y, y0, y1);
-          *reinterpret_cast<uint4*>(kh + off16<C::CH16>(k, 2 * c)) = x0;
-          *reinterpret_cast<uint4*>(kh + off16<C::CH16>(k, 2 * c + 1)) = x1;
-          *reinterpret_cast<uint4*>(kh + C::HALF_B + off16<C::CH16>(k, 2 * c)) = y0;
-          *reinterpret_cast<uint4*>(kh + C::HALF_B + off16<C::CH16>(k, 2 * c + 1)) = y1;
-        }
-      }
-      // the mask's factors with the V row's scale in them, once for all warps
-      if (gt < KT) {
-        float* cs = reinterpret_cast<float*>(ring + (size_t)slot * C::STAGE_B + 2 * C::TILE_B) + gt;
-        const float vs = cs[3 * KT];
-        cs[0] *= vs;
-        cs[KT] *= vs;
-        cs[3 * KT] = vs * 0x1p19f;
-      }
-    };
-
-    // --- the first stages, under way while the queries are brought in ------------
-    auto start = [&]() -> long long {
-      // the group's stage number `turn` sits in ring slot turn % S
-      long long rows[S];
-#pragma unroll
-      for (int i = 0; i < S; ++i) rows[i] = key_row(s0 + wk + i * C::WK);
-#pragma unroll
-      for (int i = 0; i < S - 1; ++i) load_stage(i, i, rows[i], false);
-      if (C::MG > 1 && mg == (S - 1) % C::MG) make_plan(S - 1, rows[S - 1]);
-      return rows[S - 1];
-    };
-    long long next = rg.any ? start() : -1;
-
-    // --- queries: fragments, per-row factors ------------------------------------
-    uint32_t qa[C::KS][4];
-    uint32_t ql[C::QHL ? C::KS : 1][4];
-    float rq[RH], ci[RH], si[RH];
-    int dep[RH];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (e >= RH) {
-#pragma unroll
-        for (int s = 0; s < C::KS; ++s) {
-          qa[s][1] = qa[s][3] = 0u;
-          if constexpr (C::QHL) ql[s][1] = ql[s][3] = 0u;
-        }
-        continue;
-      }
-      const int i = mg * 16 + g + 8 * e;
-      const bool in = i < a.n && rg.any;
-      const TA* q = reinterpret_cast<const TA*>(a.q) + (long long)b * a.q_sb + (long long)i * a.q_st +
-                    (long long)h * D;
-      float x[C::KS][4];
-      float ss = 0.f;
-      uint32_t top = 0;
-#pragma unroll
-      for (int s = 0; s < C::KS; ++s)
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          x[s][2 * f] = x[s][2 * f + 1] = 0.f;
-          if (in) {
-            if constexpr (sizeof(TA) == 2) {
-              const float2 v = unpack_bf16(*reinterpret_cast<const uint32_t*>(q + d_of<C>(t, s, f)));
-              x[s][2 * f] = v.x;
-              x[s][2 * f + 1] = v.y;
-            } else {
-              const float2 v = *reinterpret_cast<const float2*>(q + d_of<C>(t, s, f));
-              x[s][2 * f] = v.x;
-              x[s][2 * f + 1] = v.y;
-            }
-          }
-        }
-#pragma unroll
-      for (int s = 0; s < C::KS; ++s)
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          ss = fmaf(x[s][f], x[s][f], ss);
-          top = max(top, __float_as_uint(x[s][f]) & 0x7fffffffu);
-        }
-      ss += __shfl_xor_sync(0xffffffffu, ss, 1);
-      ss += __shfl_xor_sync(0xffffffffu, ss, 2);
-      float scale = 1.f;
-      if constexpr (C::I8) {
-        // bring the row's largest element into [1, 2): the bf16 row is then
-        // exact in fp16 (elements under 2^-16 of the largest round at 2^-25
-        // of it), an fp32 row is held as hi + lo halves to 2^-25
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        int ex = (int)(top >> 23);
-        ex = ex < 1 ? 1 : ex > 253 ? 253 : ex;
-        const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
-        scale = __uint_as_float((uint32_t)ex << 23);
-#pragma unroll
-        for (int s = 0; s < C::KS; ++s)
-#pragma unroll
-          for (int f = 0; f < 4; ++f) x[s][f] *= down;
-      }
-#pragma unroll
-      for (int s = 0; s < C::KS; ++s)
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          if constexpr (C::I8) {
-            qa[s][2 * f + e] = pack_f16(x[s][2 * f], x[s][2 * f + 1]);
-            if constexpr (C::QHL) {
-              const float2 u = __half22float2(*reinterpret_cast<__half2*>(&qa[s][2 * f + e]));
-              ql[s][2 * f + e] = pack_f16(x[s][2 * f] - u.x, x[s][2 * f + 1] - u.y);
-            }
-          } else {
-            qa[s][2 * f + e] = pack_bf16(x[s][2 * f], x[s][2 * f + 1]);
-          }
-        }
-      // S = q.k scale / max(|q|, eps), times r; scale first: 2^ex / |q| <= 1
-      rq[e] = r * (scale / fmaxf(sqrtf(ss), a.eps));
-      const bool live = in && nodes.line[i] != 0;
-      dep[e] = live ? nodes.depth[i] : 0;
-      float sn, cn;
-      sincospif((float)dep[e] / w, &sn, &cn);
-      // int8: alpha carries the V row's scale <= 1 / 127; 2^20 keeps it normal
-      // in fp16 down to alpha = 2^-23
-      ci[e] = (C::I8 ? 0x1p19f : 0.5f) * cn;
-      si[e] = (C::I8 ? 0x1p19f : 0.5f) * sn;
-      if (!live) rq[e] = __uint_as_float(0x7fc00000u);  // t = NaN: sees nothing
-    }
-    const float2 one_r = both(1.0f - r);
-
-    float o[C::NT][4];
-    // pass 0 takes every V row and scale as finite.  A non-finite one times
-    // alpha = 0 would spoil queries that do not see it: if any sum comes out
-    // non-finite, pass 1 repeats the run with such rows left out of the product
-    // and put back as NaN for the queries that see them.
 #pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {
-#pragma unroll
-      for (int j = 0; j < C::NT; ++j)
-#pragma unroll
-        for (int f = 0; f < 4; ++f) o[j][f] = 0.f;
-      if (rg.any) {
-        if (pass == 1) next = start();
-        int slot = 0, fill = S - 1, buf = 0;
+      for (int x = s0 + wk, turn = 0; x <= s1; x += C::WK, ++turn) {
+        cp_async_wait<S - 2 - AHEAD>();
+        group_sync();
+        load_stage(turn + S - 1, fill, next, true);
+        if (C::MG == 1 || mg == (turn + S) % C::MG) {
+          next = key_row(x + S * C::WK);
+          if constexpr (C::MG > 1) make_plan(turn + S, next);
+        }
+        const unsigned char* st = ring + (size_t)slot * C::STAGE_B;
+        const float* cs = reinterpret_cast<const float*>(st + 2 * C::TILE_B);
+        const int* cpos = reinterpret_cast<const int*>(cs) + (C::I8 ? 4 : 2) * KT;
+        const bool edge = cpos[KT] != 0;
+        slot = slot + 1 == S ? 0 : slot + 1;
+        fill = fill + 1 == S ? 0 : fill + 1;
+        const unsigned char *kt = st, *vt = st + C::TILE_B;
         if constexpr (C::CONV) {
-          cp_async_wait<S - 2>();
-          group_sync();
-          if (s0 + wk <= s1) widen_stage(0, 0);
+          if (x + C::WK <= s1) widen_stage(slot, buf ^ 1);
+          kt = half + (size_t)buf * 2 * C::HALF_B;
+          vt = kt + C::HALF_B;
+          buf ^= 1;
         }
-#pragma unroll 1
-        for (int x = s0 + wk, turn = 0; x <= s1; x += C::WK, ++turn) {
-          cp_async_wait<S - 2 - AHEAD>();
-          group_sync();
-          load_stage(turn + S - 1, fill, next, true);
-          if (C::MG == 1 || mg == (turn + S) % C::MG) {
-            next = key_row(x + S * C::WK);
-            if constexpr (C::MG > 1) make_plan(turn + S, next);
-          }
-          const unsigned char* st = ring + (size_t)slot * C::STAGE_B;
-          const float* cs = reinterpret_cast<const float*>(st + 2 * C::TILE_B);
-          const int* cpos = reinterpret_cast<const int*>(cs) + (C::I8 ? 4 : 2) * KT;
-          const bool edge = cpos[KT] != 0;
-          slot = slot + 1 == S ? 0 : slot + 1;
-          fill = fill + 1 == S ? 0 : fill + 1;
-          const unsigned char *kt = st, *vt = st + C::TILE_B;
-          if constexpr (C::CONV) {
-            if (x + C::WK <= s1) widen_stage(slot, buf ^ 1);
-            kt = half + (size_t)buf * 2 * C::HALF_B;
-            vt = kt + C::HALF_B;
-            buf ^= 1;
-          }
-          // --- scores of the stage: 2 NK tiles of 8 keys, each its own chain ------
-          constexpr int N8 = 2 * C::NK;
-          float2 s[N8][RH];                            // keys 2t, 2t + 1 of an 8-key tile
-          {
-            float c[N8][4], d[C::QHL ? N8 : 1][4];
-            if constexpr (C::LDM) {
+        // --- scores of the stage: 2 NK tiles of 8 keys, each its own chain ------
+        constexpr int N8 = 2 * C::NK;
+        float2 s[N8][RH];                            // keys 2t, 2t + 1 of an 8-key tile
+        {
+          float c[N8][4], d[C::QHL ? N8 : 1][4];
+          if constexpr (C::LDM) {
 #pragma unroll
-              for (int x2 = 0; x2 < C::KS; ++x2) {
-                uint32_t kb[N8][2];
+            for (int x2 = 0; x2 < C::KS; ++x2) {
+              uint32_t kb[N8][2];
 #pragma unroll
-                for (int kg = 0; kg < C::NK; ++kg) load_k16<C>(kt, kg * 16, x2, lane, kb[2 * kg], kb[2 * kg + 1]);
-                // QHL: the small products first, and apart: the tensor core's sums
-                // truncate
-                if constexpr (C::QHL) {
-#pragma unroll
-                  for (int nt = 0; nt < N8; ++nt) {
-                    if (x2 == 0) mma_first<true>(d[nt], ql[x2], kb[nt][0], kb[nt][1]);
-                    else mma_f16(d[nt], ql[x2], kb[nt][0], kb[nt][1]);
-                  }
-                }
+              for (int kg = 0; kg < C::NK; ++kg) load_k16<C>(kt, kg * 16, x2, lane, kb[2 * kg], kb[2 * kg + 1]);
+              // QHL: the small products first, and apart: the tensor core's sums
+              // truncate
+              if constexpr (C::QHL) {
 #pragma unroll
                 for (int nt = 0; nt < N8; ++nt) {
-                  if (x2 == 0) mma_first<C::I8>(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
-                  else if constexpr (C::I8) mma_f16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
-                  else mma_b16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
+                  if (x2 == 0) mma_first<true>(d[nt], ql[x2], kb[nt][0], kb[nt][1]);
+                  else mma_f16(d[nt], ql[x2], kb[nt][0], kb[nt][1]);
                 }
               }
-            } else {
-              uint32_t kb[C::NK][2][C::KS][2];
 #pragma unroll
-              for (int kg = 0; kg < C::NK; ++kg) load_k8<C>(kt, kg * 16, lane, kb[kg]);
+              for (int nt = 0; nt < N8; ++nt) {
+                if (x2 == 0) mma_first<C::I8>(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
+                else if constexpr (C::I8) mma_f16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
+                else mma_b16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
+              }
+            }
+          } else {
+            uint32_t kb[C::NK][2][C::KS][2];
 #pragma unroll
-              for (int x2 = 0; x2 < C::KS; ++x2) {
-                if constexpr (C::QHL) {
+            for (int kg = 0; kg < C::NK; ++kg) load_k8<C>(kt, kg * 16, lane, kb[kg]);
 #pragma unroll
-                  for (int nt = 0; nt < N8; ++nt) {
-                    const uint32_t* k2 = kb[nt >> 1][nt & 1][x2];
-                    if (x2 == 0) mma_first<true>(d[nt], ql[x2], k2[0], k2[1]);
-                    else mma_f16(d[nt], ql[x2], k2[0], k2[1]);
-                  }
-                }
+            for (int x2 = 0; x2 < C::KS; ++x2) {
+              if constexpr (C::QHL) {
 #pragma unroll
                 for (int nt = 0; nt < N8; ++nt) {
                   const uint32_t* k2 = kb[nt >> 1][nt & 1][x2];
-                  if (x2 == 0) mma_first<true>(c[nt], qa[x2], k2[0], k2[1]);
-                  else mma_f16(c[nt], qa[x2], k2[0], k2[1]);
+                  if (x2 == 0) mma_first<true>(d[nt], ql[x2], k2[0], k2[1]);
+                  else mma_f16(d[nt], ql[x2], k2[0], k2[1]);
                 }
               }
-            }
-            if constexpr (C::QHL) {
 #pragma unroll
-              for (int nt = 0; nt < N8; ++nt)
-#pragma unroll
-                for (int f = 0; f < 2 * RH; ++f) c[nt][f] += d[nt][f];
-            }
-#pragma unroll
-            for (int nt = 0; nt < N8; ++nt) {
-              float2 ks = both(1.f);
-              if constexpr (C::I8) ks = *reinterpret_cast<const float2*>(cs + 2 * KT + nt * 8 + 2 * t);
-#pragma unroll
-              for (int e = 0; e < RH; ++e) {
-                s[nt][e] = make_float2(c[nt][2 * e], c[nt][2 * e + 1]);
-                if constexpr (C::I8) s[nt][e] = mul2(s[nt][e], ks);
+              for (int nt = 0; nt < N8; ++nt) {
+                const uint32_t* k2 = kb[nt >> 1][nt & 1][x2];
+                if (x2 == 0) mma_first<true>(c[nt], qa[x2], k2[0], k2[1]);
+                else mma_f16(c[nt], qa[x2], k2[0], k2[1]);
               }
             }
+          }
+          if constexpr (C::QHL) {
 #pragma unroll
             for (int nt = 0; nt < N8; ++nt)
 #pragma unroll
-              for (int e = 0; e < RH; ++e) s[nt][e] = fma2(s[nt][e], both(rq[e]), one_r);
-            // NaN (an unseen row, a non-finite key) counts as 0
-#pragma unroll
-            for (int nt = 0; nt < N8; ++nt)
-#pragma unroll
-              for (int e = 0; e < RH; ++e)
-                s[nt][e] = make_float2(fmaxf(s[nt][e].x, 0.f), fmaxf(s[nt][e].y, 0.f));
+              for (int f = 0; f < 2 * RH; ++f) c[nt][f] += d[nt][f];
           }
-          if (edge) {
-#pragma unroll
-            for (int nt = 0; nt < N8; ++nt)
-#pragma unroll
-              for (int f = 0; f < 2; ++f) {
-                const int c = cpos[nt * 8 + 2 * t + f];
-                const long long at = (long long)x * KT + nt * 8 + key_of<C>(2 * t + f) - lens;
-#pragma unroll
-                for (int e = 0; e < RH; ++e) {
-                  bool see = dep[e] - c <= rg.dmax;
-                  const int i = mg * 16 + g + 8 * e;
-                  if (at >= 0 && at < a.n && i < a.n) see = see && (nodes.line[i] >> at & 1);
-                  if (!see) (f ? s[nt][e].y : s[nt][e].x) = 0.f;
-                }
-              }
-          }
-          // a lone warp skips the alpha V of 16 keys that are all under the trim; of
-          // several warps' queries some nearly always see one
-          bool live[C::NK];
-#pragma unroll
-          for (int kg = 0; kg < C::NK; ++kg) {
-            float tmax = 0.f;
-#pragma unroll
-            for (int nt = 2 * kg; nt < 2 * kg + 2; ++nt)
-#pragma unroll
-              for (int e = 0; e < RH; ++e) tmax = fmaxf(tmax, fmaxf(s[nt][e].x, s[nt][e].y));
-            live[kg] = C::MG > 1 || __any_sync(0xffffffffu, tmax > 0.f);
-          }
-          // --- alpha = t^2 (1 + cos) / 2, times the V row's scale -------------------
-          float2 al[N8][RH];
 #pragma unroll
           for (int nt = 0; nt < N8; ++nt) {
-            float2 cc = *reinterpret_cast<const float2*>(cs + nt * 8 + 2 * t);
-            float2 sc = *reinterpret_cast<const float2*>(cs + KT + nt * 8 + 2 * t);
-            float2 hc = both(0.5f);
-            if constexpr (C::I8) {
-              const float2 vs = *reinterpret_cast<const float2*>(cs + 3 * KT + nt * 8 + 2 * t);
-              if constexpr (C::CONV) {
-                hc = vs;
-              } else {
-                cc = mul2(cc, vs);
-                sc = mul2(sc, vs);
-                hc = mul2(vs, both(0x1p19f));
-              }
+            float2 ks = both(1.f);
+            if constexpr (C::I8) ks = *reinterpret_cast<const float2*>(cs + 2 * KT + nt * 8 + 2 * t);
+#pragma unroll
+            for (int e = 0; e < RH; ++e) {
+              s[nt][e] = make_float2(c[nt][2 * e], c[nt][2 * e + 1]);
+              if constexpr (C::I8) s[nt][e] = mul2(s[nt][e], ks);
             }
-#pragma unroll
-            for (int e = 0; e < RH; ++e) al[nt][e] = fma2(sc, both(si[e]), hc);
-#pragma unroll
-            for (int e = 0; e < RH; ++e) al[nt][e] = fma2(cc, both(ci[e]), al[nt][e]);
           }
 #pragma unroll
           for (int nt = 0; nt < N8; ++nt)
 #pragma unroll
-            for (int e = 0; e < RH; ++e) al[nt][e] = mul2(mul2(s[nt][e], s[nt][e]), al[nt][e]);
-          // pass 1: V rows with a non-finite value (bit: score column) leave the
-          // product; a query that sees one gets NaN
-          uint32_t bad = 0;
-          if (pass == 1) {
-            bool nf = false;
-            if (lane < KT) {
-              if constexpr (C::I8) {
-                nf = !(fabsf(cs[3 * KT + lane]) < 3.0e38f);
-              } else {
-                for (int c = 0; c < C::CH; ++c) {
-                  const uint4 u = *reinterpret_cast<const uint4*>(vt + v_off<C>(lane, c));
-                  const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
+            for (int e = 0; e < RH; ++e) s[nt][e] = fma2(s[nt][e], both(rq[e]), one_r);
+          // NaN (an unseen row, a non-finite key) counts as 0
 #pragma unroll
-                  for (int q = 0; q < 4; ++q)
-                    nf = nf || (ww[q] & 0x7f80u) == 0x7f80u || (ww[q] & 0x7f800000u) == 0x7f800000u;
-                }
-              }
-            }
-            bad = __ballot_sync(0xffffffffu, nf);
-            if (bad) {
+          for (int nt = 0; nt < N8; ++nt)
 #pragma unroll
-              for (int nt = 0; nt < N8; ++nt)
+            for (int e = 0; e < RH; ++e)
+              s[nt][e] = make_float2(fmaxf(s[nt][e].x, 0.f), fmaxf(s[nt][e].y, 0.f));
+        }
+        if (edge) {
 #pragma unroll
-                for (int e = 0; e < RH; ++e) {
-                  const uint32_t two = bad >> (8 * nt + 2 * t);
-                  const float2 x1 = s[nt][e];
-                  if (((two & 1) && x1.x > 0.f) || ((two & 2) && x1.y > 0.f))
-                    o[0][2 * e] = __uint_as_float(0x7fc00000u);
-                  if (two & 1) al[nt][e].x = 0.f;
-                  if (two & 2) al[nt][e].y = 0.f;
-                }
-            }
-          }
-          // --- alpha V, 16 keys at a time -------------------------------------------
+          for (int nt = 0; nt < N8; ++nt)
 #pragma unroll
-          for (int kg = 0; kg < C::NK; ++kg) {
-            if (!live[kg]) continue;
-            // a fragment's registers: row half e of 8-key tile nt
-            uint32_t pa[4] = {0u, 0u, 0u, 0u}, pl[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
+            for (int f = 0; f < 2; ++f) {
+              const int c = cpos[nt * 8 + 2 * t + f];
+              const long long at = (long long)x * KT + nt * 8 + key_of<C>(2 * t + f) - lens;
 #pragma unroll
               for (int e = 0; e < RH; ++e) {
-                const int f = 2 * nt + e;
-                const float2 v = al[2 * kg + nt][e];
-                pa[f] = C::I8 ? pack_f16(v.x, v.y) : pack_bf16(v.x, v.y);
-                if constexpr (C::PHL) {
-                  const float2 u = C::I8 ? __half22float2(*reinterpret_cast<__half2*>(&pa[f]))
-                                         : unpack_bf16(pa[f]);
-                  pl[f] = C::I8 ? pack_f16(v.x - u.x, v.y - u.y) : pack_bf16(v.x - u.x, v.y - u.y);
-                }
-              }
-            uint32_t vb[C::NT][2];
-            load_v<C>(vt, kg * 16, lane, vb);
-            if constexpr (!C::I8) {
-              if (bad) {
-#pragma unroll
-                for (int j = 0; j < C::NT; ++j)
-#pragma unroll
-                  for (int hh = 0; hh < 2; ++hh) {
-                    const uint32_t two = bad >> (16 * kg + 8 * hh + 2 * t);
-                    if (two & 1) vb[j][hh] &= 0xffff0000u;
-                    if (two & 2) vb[j][hh] &= 0x0000ffffu;
-                  }
+                bool see = dep[e] - c <= rg.dmax;
+                const int i = mg * 16 + g + 8 * e;
+                if (at >= 0 && at < a.n && i < a.n) see = see && (nodes.line[i] >> at & 1);
+                if (!see) (f ? s[nt][e].y : s[nt][e].x) = 0.f;
               }
             }
-            if constexpr (C::QHL) {
+        }
+        // a lone warp skips the alpha V of 16 keys that are all under the trim; of
+        // several warps' queries some nearly always see one
+        bool live[C::NK];
 #pragma unroll
-              for (int j = 0; j < C::NT; ++j) {
-                float d[4];
-                mma_first<true>(d, pl, vb[j][0], vb[j][1]);
-                mma_f16(d, pa, vb[j][0], vb[j][1]);
+        for (int kg = 0; kg < C::NK; ++kg) {
+          float tmax = 0.f;
 #pragma unroll
-                for (int f = 0; f < 2 * RH; ++f) o[j][f] += d[f];
-              }
-            } else if constexpr (C::I8) {
+          for (int nt = 2 * kg; nt < 2 * kg + 2; ++nt)
 #pragma unroll
-              for (int j = 0; j < C::NT; ++j) mma_f16(o[j], pa, vb[j][0], vb[j][1]);
+            for (int e = 0; e < RH; ++e) tmax = fmaxf(tmax, fmaxf(s[nt][e].x, s[nt][e].y));
+          live[kg] = C::MG > 1 || __any_sync(0xffffffffu, tmax > 0.f);
+        }
+        // --- alpha = t^2 (1 + cos) / 2, times the V row's scale -------------------
+        float2 al[N8][RH];
+#pragma unroll
+        for (int nt = 0; nt < N8; ++nt) {
+          float2 cc = *reinterpret_cast<const float2*>(cs + nt * 8 + 2 * t);
+          float2 sc = *reinterpret_cast<const float2*>(cs + KT + nt * 8 + 2 * t);
+          float2 hc = both(0.5f);
+          if constexpr (C::I8) {
+            const float2 vs = *reinterpret_cast<const float2*>(cs + 3 * KT + nt * 8 + 2 * t);
+            if constexpr (C::CONV) {
+              hc = vs;
             } else {
-#pragma unroll
-              for (int j = 0; j < C::NT; ++j) mma_b16(o[j], pl, vb[j][0], vb[j][1]);
-#pragma unroll
-              for (int j = 0; j < C::NT; ++j) mma_b16(o[j], pa, vb[j][0], vb[j][1]);
+              cc = mul2(cc, vs);
+              sc = mul2(sc, vs);
+              hc = mul2(vs, both(0x1p19f));
             }
           }
+#pragma unroll
+          for (int e = 0; e < RH; ++e) al[nt][e] = fma2(sc, both(si[e]), hc);
+#pragma unroll
+          for (int e = 0; e < RH; ++e) al[nt][e] = fma2(cc, both(ci[e]), al[nt][e]);
         }
-        cp_async_wait<0>();
+#pragma unroll
+        for (int nt = 0; nt < N8; ++nt)
+#pragma unroll
+          for (int e = 0; e < RH; ++e) al[nt][e] = mul2(mul2(s[nt][e], s[nt][e]), al[nt][e]);
+        // pass 1: V rows with a non-finite value (bit: score column) leave the
+        // product; a query that sees one gets NaN
+        uint32_t bad = 0;
+        if (pass == 1) {
+          bool nf = false;
+          if (lane < KT) {
+            if constexpr (C::I8) {
+              nf = !(fabsf(cs[3 * KT + lane]) < 3.0e38f);
+            } else {
+              for (int c = 0; c < C::CH; ++c) {
+                const uint4 u = *reinterpret_cast<const uint4*>(vt + v_off<C>(lane, c));
+                const uint32_t ww[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  nf = nf || (ww[q] & 0x7f80u) == 0x7f80u || (ww[q] & 0x7f800000u) == 0x7f800000u;
+              }
+            }
+          }
+          bad = __ballot_sync(0xffffffffu, nf);
+          if (bad) {
+#pragma unroll
+            for (int nt = 0; nt < N8; ++nt)
+#pragma unroll
+              for (int e = 0; e < RH; ++e) {
+                const uint32_t two = bad >> (8 * nt + 2 * t);
+                const float2 x1 = s[nt][e];
+                if (((two & 1) && x1.x > 0.f) || ((two & 2) && x1.y > 0.f))
+                  o[0][2 * e] = __uint_as_float(0x7fc00000u);
+                if (two & 1) al[nt][e].x = 0.f;
+                if (two & 2) al[nt][e].y = 0.f;
+              }
+          }
+        }
+        // --- alpha V, 16 keys at a time -------------------------------------------
+#pragma unroll
+        for (int kg = 0; kg < C::NK; ++kg) {
+          if (!live[kg]) continue;
+          // a fragment's registers: row half e of 8-key tile nt
+          uint32_t pa[4] = {0u, 0u, 0u, 0u}, pl[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < RH; ++e) {
+              const int f = 2 * nt + e;
+              const float2 v = al[2 * kg + nt][e];
+              pa[f] = C::I8 ? pack_f16(v.x, v.y) : pack_bf16(v.x, v.y);
+              if constexpr (C::PHL) {
+                const float2 u = C::I8 ? __half22float2(*reinterpret_cast<__half2*>(&pa[f]))
+                                       : unpack_bf16(pa[f]);
+                pl[f] = C::I8 ? pack_f16(v.x - u.x, v.y - u.y) : pack_bf16(v.x - u.x, v.y - u.y);
+              }
+            }
+          uint32_t vb[C::NT][2];
+          load_v<C>(vt, kg * 16, lane, vb);
+          if constexpr (!C::I8) {
+            if (bad) {
+#pragma unroll
+              for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                  const uint32_t two = bad >> (16 * kg + 8 * hh + 2 * t);
+                  if (two & 1) vb[j][hh] &= 0xffff0000u;
+                  if (two & 2) vb[j][hh] &= 0x0000ffffu;
+                }
+            }
+          }
+          if constexpr (C::QHL) {
+#pragma unroll
+            for (int j = 0; j < C::NT; ++j) {
+              float d[4];
+              mma_first<true>(d, pl, vb[j][0], vb[j][1]);
+              mma_f16(d, pa, vb[j][0], vb[j][1]);
+#pragma unroll
+              for (int f = 0; f < 2 * RH; ++f) o[j][f] += d[f];
+            }
+          } else if constexpr (C::I8) {
+#pragma unroll
+            for (int j = 0; j < C::NT; ++j) mma_f16(o[j], pa, vb[j][0], vb[j][1]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < C::NT; ++j) mma_b16(o[j], pl, vb[j][0], vb[j][1]);
+#pragma unroll
+            for (int j = 0; j < C::NT; ++j) mma_b16(o[j], pa, vb[j][0], vb[j][1]);
+          }
+        }
       }
-      bool nf = false;
-#pragma unroll
-      for (int j = 0; j < C::NT; ++j)
-#pragma unroll
-        for (int f = 0; f < 2 * RH; ++f) nf = nf || !(fabsf(o[j][f]) < 3.0e38f);
-      if (!__syncthreads_or(nf)) break;
+      cp_async_wait<0>();
     }
-    __syncthreads();   // the rings become the reduction buffer
+    bool nf = false;
+#pragma unroll
+    for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+      for (int f = 0; f < 2 * RH; ++f) nf = nf || !(fabsf(o[j][f]) < 3.0e38f);
+    if (!__syncthreads_or(nf)) break;
+  }
+  __syncthreads();   // the rings become the reduction buffer
 
-    // --- sum the groups, finish or leave the partial ----------------------------
-    float* red = reinterpret_cast<float*>(dsm);          // [WK][MG * 16][D]
-    constexpr int ROWS = C::MG * 16;
+  // --- sum the groups, finish or leave the partial ----------------------------
+  float* red = reinterpret_cast<float*>(dsm);          // [WK][MG * 16][D]
+  constexpr int ROWS = C::MG * 16;
 #pragma unroll
-    for (int e = 0; e < RH; ++e) {
-      float* dst = red + ((size_t)wk * ROWS + mg * 16 + g + 8 * e) * D;
+  for (int e = 0; e < RH; ++e) {
+    float* dst = red + ((size_t)wk * ROWS + mg * 16 + g + 8 * e) * D;
 #pragma unroll
-      for (int j = 0; j < C::NT; ++j)
+    for (int j = 0; j < C::NT; ++j)
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
-          dst[o_col<C>(j, 2 * t + f)] = C::I8 ? o[j][2 * e + f] * 0x1p-20f : o[j][2 * e + f];
-    }
-    __syncthreads();
-    if (!whole) {
-      float4* dst = reinterpret_cast<float4*>(part + (size_t)(blockIdx.x + sh.seg) * a.n * D);
-      for (int u = tid; u < a.n * (D / 4); u += kThreads) {
-        float4 x = reinterpret_cast<const float4*>(red)[u];
+      for (int f = 0; f < 2; ++f)
+        dst[o_col<C>(j, 2 * t + f)] = C::I8 ? o[j][2 * e + f] * 0x1p-20f : o[j][2 * e + f];
+  }
+  __syncthreads();
+  if (!whole) {
+    float4* dst = reinterpret_cast<float4*>(part + (size_t)blockIdx.x * a.n * D);
+    for (int u = tid; u < a.n * (D / 4); u += kThreads) {
+      float4 x = reinterpret_cast<const float4*>(red)[u];
 #pragma unroll
-        for (int k = 1; k < C::WK; ++k) {
-          const float4 y = reinterpret_cast<const float4*>(red + (size_t)k * ROWS * D)[u];
-          x.x += y.x;
-          x.y += y.y;
-          x.z += y.z;
-          x.w += y.w;
-        }
-        dst[u] = x;
+      for (int k = 1; k < C::WK; ++k) {
+        const float4 y = reinterpret_cast<const float4*>(red + (size_t)k * ROWS * D)[u];
+        x.x += y.x;
+        x.y += y.y;
+        x.z += y.z;
+        x.w += y.w;
       }
-      continue;
+      dst[u] = x;
     }
-    constexpr int PER = D < 32 ? 1 : D / 32;
-    for (int i = warp; i < a.n; i += 4) {
-      float x[PER];
+    return;
+  }
+  constexpr int PER = D < 32 ? 1 : D / 32;
+  for (int i = warp; i < a.n; i += 4) {
+    float x[PER];
 #pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        x[e] = 0.f;
-        if (lane + 32 * e < D)
+    for (int e = 0; e < PER; ++e) {
+      x[e] = 0.f;
+      if (lane + 32 * e < D)
 #pragma unroll
-          for (int k = 0; k < C::WK; ++k) x[e] += red[((size_t)k * ROWS + i) * D + lane + 32 * e];
-      }
-      store_row<TA, D>(a, b, i, h, lane, x, rg.any && nodes.line[i] != 0);
+        for (int k = 0; k < C::WK; ++k) x[e] += red[((size_t)k * ROWS + i) * D + lane + 32 * e];
     }
+    store_row<TA, D>(a, b, i, h, lane, x, rg.any && nodes.line[i] != 0);
   }
 }
 
