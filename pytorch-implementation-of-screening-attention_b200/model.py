@@ -16,6 +16,7 @@ from . import _lib
 from .functional import cross_entropy, rms_eps, rms_norm
 from .kv_cache import PagedKVCache
 from .layers import MultiscreenBlock
+from .paged import MAX_NODES, tree_depths, verify_drafts
 from .sequence_parallel import current_shard
 
 
@@ -35,6 +36,14 @@ def _sharded_mean_ce(logits, labels, shard):
 
 
 _rms_eps = rms_eps
+
+
+def _keep_top(logits: torch.Tensor, top_k: int | None) -> torch.Tensor:
+    """logits with everything under the k-th largest of a row at -inf (model.py:136-138)."""
+    if top_k is None:
+        return logits
+    least = torch.topk(logits, top_k).values[..., -1:]
+    return logits.masked_fill(logits < least, float("-inf"))
 
 
 class MultiscreenLM(nn.Module):
@@ -113,13 +122,15 @@ class MultiscreenLM(nn.Module):
         return float(ws.max()) if ws.numel() else 0.0
 
     def make_cache(self, batch: int, max_len: int, dtype: torch.dtype | None = None,
-                   page_size: int = 64) -> PagedKVCache:
+                   page_size: int = 64, quantize: str | None = None,
+                   max_draft: int = 0) -> PagedKVCache:
         a0 = self.blocks[0].attn
         dt = dtype or self.token_emb.weight.dtype
         if dt not in (torch.float32, torch.bfloat16):
             dt = torch.float32
         return PagedKVCache(len(self.blocks), batch, a0.num_heads, a0.head_dim, max_len,
-                            self._max_window(), dt, self.token_emb.weight.device, page_size)
+                            self._max_window(), dt, self.token_emb.weight.device, page_size,
+                            quantize, max_draft)
 
     @torch.no_grad()
     def prefill(self, input_ids: torch.Tensor, cache: PagedKVCache | None) -> torch.Tensor:
@@ -139,11 +150,13 @@ class MultiscreenLM(nn.Module):
 
     @torch.no_grad()
     def decode_step(self, tokens: torch.Tensor, position, cache: PagedKVCache,
-                    state: dict | None = None) -> torch.Tensor:
+                    state: dict | None = None, clamp_position: bool = False) -> torch.Tensor:
         """tokens (B,1) at absolute `position` (an int, or an int32 (B,) device
         tensor); returns logits (B,V).  With a tensor position the step has no
         host-side dependence on the position, so it can be captured once in a
-        CUDA graph and replayed for every generated token."""
+        CUDA graph and replayed for every generated token.  clamp_position: a
+        position past max_seq_len takes the last position embedding (drafts past
+        the end of a text, whose tokens are dropped)."""
         B = tokens.shape[0]
         dev = tokens.device
         if state is None:
@@ -152,7 +165,10 @@ class MultiscreenLM(nn.Module):
             pos_t = position
         else:
             pos_t = torch.full((B,), position, dtype=torch.int32, device=dev)
-        x = self.token_emb(tokens) + self.pos_emb(pos_t.long()).unsqueeze(1)
+        at = pos_t.long()
+        if clamp_position:
+            at = at.clamp_max(self.pos_emb.num_embeddings - 1)
+        x = self.token_emb(tokens) + self.pos_emb(at).unsqueeze(1)
         seq_lens = pos_t + 1
         if self._rows_fast(x):
             # few tokens: every linear layer is one bandwidth-bound pass over
@@ -174,6 +190,52 @@ class MultiscreenLM(nn.Module):
             x = x + blk.attn.decode_step(blk.norm1(x), cache, li, pos_t, seq_lens, wqkv, r, w)
             x = x + blk.ffn(blk.norm2(x))
         return self.lm_head(self.norm(x))[:, -1]
+
+    @torch.no_grad()
+    def tree_step(self, tokens: torch.Tensor, lens: torch.Tensor, cache: PagedKVCache,
+                  parents: torch.Tensor | None = None, depths: torch.Tensor | None = None,
+                  state: dict | None = None) -> torch.Tensor:
+        """Logits (B,n,V) of a tree of n tokens per sequence behind the lens[b]
+        (int32) tokens in `cache` (make_cache(max_draft >= n - 1)); their keys and
+        values are left in the cache at lens[b] + i.  parents as in
+        paged_tree_decode, None for a chain; depths (B,n): the nodes' depths if
+        they are at hand.  Node i of a chain sees what decode_step would at
+        position lens[b] + i.  After verify_drafts, cache.commit keeps the
+        accepted path (a chain's is in place)."""
+        B, n = tokens.shape
+        if state is None:
+            state = self._decode_state()
+        if depths is None:
+            depths = (torch.arange(n, device=tokens.device).expand(B, n) if parents is None
+                      else tree_depths(parents))
+        pos = (lens.long().clamp_min(0).unsqueeze(1) + depths).clamp_max(
+            self.pos_emb.num_embeddings - 1)
+        x = self.token_emb(tokens.clamp_min(0)) + self.pos_emb(pos)
+        a0 = self.blocks[0].attn
+        H, D, d = a0.num_heads, a0.head_dim, self.d_model
+        fast = B * n <= 8 and self._rows_fast(x.reshape(B * n, 1, d))
+        h = x.reshape(B * n, d) if fast else x
+        for li, blk in enumerate(self.blocks):
+            wqkv, r, w = state["layers"][li]
+            if fast:
+                qkv = _lib.rows_linear(h, wqkv, norm_w=blk.norm1.weight, eps=_rms_eps(blk.norm1, h))
+            else:
+                qkv = F.linear(rms_norm(blk.norm1, h), wqkv)
+            qkv = qkv.view(B, n, 3, H, D)
+            y = cache.append_tree_decode(li, qkv[:, :, 1], qkv[:, :, 2], qkv[:, :, 0], lens, parents,
+                                         r, w, eps=blk.attn.eps)
+            if fast:
+                h = _lib.rows_linear(y.view(B * n, d), blk.attn.out_proj.weight, res=h)
+                u = _lib.rows_linear(h, blk.ffn[0].weight, norm_w=blk.norm2.weight,
+                                     eps=_rms_eps(blk.norm2, h), act=1)
+                h = _lib.rows_linear(u, blk.ffn[3].weight, res=h)
+            else:
+                h = h + blk.attn.out_proj(y.view(B, n, d).to(h.dtype))
+                h = h + blk.ffn(rms_norm(blk.norm2, h))
+        if fast:
+            return _lib.rows_linear(h, self.lm_head.weight, norm_w=self.norm.weight,
+                                    eps=_rms_eps(self.norm, h)).view(B, n, -1)
+        return self._lm_logits(rms_norm(self.norm, h))[0]
 
     def _rows_fast(self, x: torch.Tensor) -> bool:
         """The fused few-row decode path applies: bf16 CUDA weights and
@@ -224,10 +286,11 @@ class MultiscreenLM(nn.Module):
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int = 100,
                  temperature: float = 1.0, top_k: int | None = None,
-                 cuda_graph: bool = True) -> torch.Tensor:
+                 cuda_graph: bool = True, cache_quantize: str | None = None) -> torch.Tensor:
         """(B,T) prompt -> (B, T + max_new_tokens), sampling as model.py:134-140.
         On CUDA the per-token decode step is one CUDA-graph replay
-        (`cuda_graph=False`: eager launches, same numbers)."""
+        (`cuda_graph=False`: eager launches, same numbers).  cache_quantize="int8"
+        keeps the cached keys and values in 8 bits."""
         self.eval()
         if max_new_tokens <= 0:
             return input_ids
@@ -235,7 +298,7 @@ class MultiscreenLM(nn.Module):
         if T0 + max_new_tokens - 1 > self.pos_emb.num_embeddings:
             # the reference fails the same way inside pos_emb (model.py:90-92)
             raise IndexError("index out of range in self: prompt + new tokens exceed max_seq_len")
-        cache = self.make_cache(B, T0 + max_new_tokens)
+        cache = self.make_cache(B, T0 + max_new_tokens, quantize=cache_quantize)
         state = self._decode_state()
         logits = self.prefill(input_ids, cache)
         graph = None
@@ -258,3 +321,101 @@ class MultiscreenLM(nn.Module):
                 else:
                     logits = self.decode_step(next_token, T0 + step, cache, state)
         return input_ids
+
+    # ------------------------------------------------------------------
+    def _speculate(self, draft: "MultiscreenLM", last: torch.Tensor, lens: torch.Tensor,
+                   uniforms: torch.Tensor, num_draft: int, caches, states, temperature: float,
+                   top_k: int | None):
+        """One round: num_draft tokens drawn from `draft` one by one after `last`
+        (B,1), all verified by one tree step of this model.  uniforms (B,
+        2 num_draft + 1).  Returns verify_drafts' (tokens, counts)."""
+        B = last.shape[0]
+        none = last.new_empty((B, 0))
+        tokens, rows = [last], []
+        for i in range(num_draft + 1):
+            # the last draft's step only leaves its row in the drafting cache
+            lg = draft.decode_step(tokens[-1], lens + i, caches[1], states[1], clamp_position=True)
+            if i < num_draft:
+                lg = _keep_top(lg, top_k)
+                rows.append(lg)
+                drawn, _, _ = verify_drafts(lg.unsqueeze(1), none, None, uniforms[:, i:i + 1],
+                                            temperature=temperature)
+                tokens.append(drawn)
+        chain = torch.cat(tokens, 1)
+        logits = _keep_top(self.tree_step(chain, lens, caches[0], state=states[0]), top_k)
+        out, _, counts = verify_drafts(logits, chain[:, 1:], None, uniforms[:, num_draft:],
+                                       draft_logits=torch.stack(rows, 1).to(logits.dtype),
+                                       temperature=temperature)
+        return out, counts
+
+    @torch.no_grad()
+    def generate_speculative(self, input_ids: torch.Tensor, draft: "MultiscreenLM",
+                             max_new_tokens: int = 100, num_draft: int = 4,
+                             temperature: float = 1.0, top_k: int | None = None,
+                             cuda_graph: bool = True, cache_quantize: str | None = None,
+                             generator: torch.Generator | None = None) -> torch.Tensor:
+        """generate() with `draft` (a smaller model over the same vocabulary)
+        proposing num_draft tokens a round, which this model verifies in one step:
+        the tokens are distributed as generate()'s (temperature 0: this model's
+        greedy tokens), a round yields 1 to num_draft + 1 of them per sequence.
+        On CUDA a round is one CUDA-graph replay."""
+        self.eval()
+        draft.eval()
+        if max_new_tokens <= 0:
+            return input_ids
+        B, T0 = input_ids.shape
+        if not 1 <= num_draft < MAX_NODES:
+            raise ValueError(f"num_draft must be in [1, {MAX_NODES - 1}]")
+        if draft.token_emb.num_embeddings != self.token_emb.num_embeddings:
+            raise ValueError("the drafting model has another vocabulary")
+        for m in (self, draft):
+            if T0 + max_new_tokens - 1 > m.pos_emb.num_embeddings:
+                raise IndexError("index out of range in self: prompt + new tokens exceed max_seq_len")
+        dev = input_ids.device
+        # a finished sequence is drafted past its end; what it yields is dropped
+        room = T0 + max_new_tokens + num_draft + 1
+        caches = [m.make_cache(B, room, quantize=cache_quantize, max_draft=num_draft)
+                  for m in (self, draft)]
+        states = [self._decode_state(), draft._decode_state()]
+        logits = _keep_top(self.prefill(input_ids, caches[0]), top_k)
+        draft.prefill(input_ids, caches[1])
+
+        def draw(n):
+            return torch.rand(B, n, device=dev, generator=generator)
+
+        last, _, _ = verify_drafts(logits.unsqueeze(1), input_ids.new_empty((B, 0)), None, draw(1),
+                                   temperature=temperature)
+        lens = torch.full((B,), T0, dtype=torch.int32, device=dev)
+        made = torch.ones(B, dtype=torch.long, device=dev)
+        new = torch.zeros(B, max_new_tokens + num_draft + 1, dtype=torch.long, device=dev)
+        new[:, 0] = last[:, 0]
+        uniforms = draw(2 * num_draft + 1)
+        args = (draft, last, lens, uniforms, num_draft, caches, states, temperature, top_k)
+        graph = None
+        if cuda_graph and input_ids.is_cuda and max_new_tokens > 1:
+            # the rows that the warm-up and the capture write are written again by
+            # the first round
+            side = torch.cuda.Stream(device=dev)
+            side.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(side):
+                self._speculate(*args)
+            torch.cuda.current_stream(dev).wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out, counts = self._speculate(*args)
+        step = torch.arange(num_draft + 1, device=dev)
+        while int(made.min()) < max_new_tokens:
+            if graph is not None:
+                graph.replay()
+            else:
+                out, counts = self._speculate(*args)
+            going = made < max_new_tokens
+            got = torch.where(going, counts.long() + 1, 0)
+            at = (made.unsqueeze(1) + step).clamp_max(new.shape[1] - 1)
+            keep = step < got.unsqueeze(1)
+            new.scatter_(1, at, torch.where(keep, out, new.gather(1, at)))
+            last.copy_(torch.where(going.unsqueeze(1), out.gather(1, counts.long().unsqueeze(1)), last))
+            lens.add_(got.to(torch.int32))
+            made = made + got
+            uniforms.copy_(draw(2 * num_draft + 1))
+        return torch.cat([input_ids, new[:, :max_new_tokens]], 1)

@@ -351,6 +351,23 @@ def paged_tree_decode(q, k, v, lens, parents, r, w, k_pages, v_pages, block_tabl
                  k_scales, v_scales, max_window, num_ctas, eps)
 
 
+def tree_depths(parents):
+    """Depth (B, n) int64 of every node of parents (B, n): 0 below the newest cached
+    token.  Absent nodes have a depth without meaning."""
+    p = parents.long()
+    B, n = p.shape
+    p = torch.where((p >= 0) & (p < torch.arange(n, device=p.device)), p, -1)
+    depth = (p >= 0).long()
+    hop = 1
+    while hop < n:                        # pointer doubling
+        at = p.clamp_min(0)
+        inner = p >= 0
+        depth = depth + torch.where(inner, depth.gather(1, at), 0)
+        p = torch.where(inner, p.gather(1, at), -1)
+        hop *= 2
+    return depth
+
+
 def paged_commit(lens, path, counts, k_pages, v_pages, block_table, k_scales=None,
                  v_scales=None) -> None:
     """Keep an accepted path: row lens[b] + path[b, i] moves to lens[b] + i for
