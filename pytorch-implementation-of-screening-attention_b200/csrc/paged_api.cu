@@ -143,7 +143,7 @@ int screen_paged_commit(const screen_commit_args* a, screen_stream_t stream) {
     return SCREEN_ERR_INVALID_ARG;
   if ((long long)a->L * a->B * a->H * a->n == 0) return SCREEN_OK;
   if (!a->lens || !a->path || !a->counts) return SCREEN_ERR_INVALID_ARG;
-  if (a->L > 65535) return SCREEN_ERR_UNSUPPORTED;
+  if (a->L > 65535 || (long long)a->B * a->H > (1 << 28)) return SCREEN_ERR_UNSUPPORTED;
   int st = cache_ok(a->cache, a->cache_dtype, a->k_scales, a->v_scales);
   if (st) return st;
   commit(*a, (cudaStream_t)stream);

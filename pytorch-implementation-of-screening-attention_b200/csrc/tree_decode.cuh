@@ -56,7 +56,12 @@ __device__ __forceinline__ Range tree_range(const TreeParams& p, int b, int h) {
   g.first = g.lens - (g.dmax > 0 ? g.dmax : 0);
   if (g.first < 0) g.first = 0;
   g.t0 = (int)(g.first / kTile);
-  g.nt = (int)((g.lens + p.a.n - 1) / kTile) - g.t0 + 1;
+  // no key stands past the end of the block table
+  const long long rows = (long long)p.a.cache.max_blocks * p.a.cache.page_size;
+  long long last = g.lens + p.a.n - 1;
+  if (last > rows - 1) last = rows - 1;
+  g.nt = (int)(last / kTile) - g.t0 + 1;
+  if (g.nt < 1) g.nt = 1;
   return g;
 }
 

@@ -308,7 +308,12 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
   bool whole;
   if (!find_run(p, reinterpret_cast<int*>(dsm), slots, seg, rg, c0, c1, whole)) return;
   const int b = seg / a.H, h = seg % a.H;
-  const float w = a.w[h], r = a.r[h];
+  // w <= 1 sees the query's own position alone, where the mask is 1 whatever w is;
+  // 0, a NaN or a tiny w would put a NaN into the factors of its cosine
+  const float w = fmaxf(a.w[h], 1.f), r = a.r[h];
+  // r < 0 turns alpha up to (1 + 2 |r|)^2: t is held down by a power of two, so
+  // that alpha stays below 4 (fp16 holds alpha * 2^20 / 127 up to alpha = 7.9)
+  const float up = r < 0.f ? __uint_as_float(__float_as_uint(1.f - 2.f * r) & 0x7f800000u) : 1.f;
   const long long lens = rg.lens;
   if (warp == 0) tree_nodes(a, b, nodes, lane);
   __syncthreads();
@@ -534,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
         }
       }
     // S = q.k scale / max(|q|, eps), times r; scale first: 2^ex / |q| <= 1
-    rq[e] = r * (scale / fmaxf(sqrtf(ss), a.eps));
+    rq[e] = r / up * (scale / fmaxf(sqrtf(ss), a.eps));
     const bool live = in && nodes.line[i] != 0;
     dep[e] = live ? nodes.depth[i] : 0;
     float sn, cn;
@@ -545,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
     si[e] = (C::I8 ? 0x1p19f : 0.5f) * sn;
     if (!live) rq[e] = __uint_as_float(0x7fc00000u);  // t = NaN: sees nothing
   }
-  const float2 one_r = both(1.0f - r);
+  const float2 one_r = both((1.0f - r) / up);
 
   float o[C::NT][4];
   // pass 0 takes every V row and scale as finite.  A non-finite one times
@@ -818,6 +823,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
   // --- sum the groups, finish or leave the partial ----------------------------
   float* red = reinterpret_cast<float*>(dsm);          // [WK][MG * 16][D]
   constexpr int ROWS = C::MG * 16;
+  const float back = (C::I8 ? 0x1p-20f : 1.f) * up * up;
 #pragma unroll
   for (int e = 0; e < RH; ++e) {
     float* dst = red + ((size_t)wk * ROWS + mg * 16 + g + 8 * e) * D;
@@ -825,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
     for (int j = 0; j < C::NT; ++j)
 #pragma unroll
       for (int f = 0; f < 2; ++f)
-        dst[o_col<C>(j, 2 * t + f)] = C::I8 ? o[j][2 * e + f] * 0x1p-20f : o[j][2 * e + f];
+        dst[o_col<C>(j, 2 * t + f)] = o[j][2 * e + f] * back;
   }
   __syncthreads();
   if (!whole) {

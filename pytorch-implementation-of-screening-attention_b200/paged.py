@@ -158,7 +158,8 @@ def _rows(x, shape, index, name):
     vec = 8 if x.dtype is torch.bfloat16 else 4
     p = x.data_ptr()
     if sd != 1 or sh != shape[3] or sb % vec or st % vec or p % 16:
-        x = x.detach().contiguous()
+        # a copy even where torch counts x as contiguous: it may start anywhere
+        x = x.detach().clone(memory_format=torch.contiguous_format)
         sb, st, _, _ = x.stride()
         p = x.data_ptr()
     return x, p, sb, st
@@ -254,7 +255,7 @@ def _tree(name, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_s
             raise ValueError(f"q must have shape {full}, got {tuple(q.shape)}")
         q_sb, sh, sd = q.stride()
         if sd != 1 or sh != D or q_sb % (8 if q.dtype is torch.bfloat16 else 4) or q.data_ptr() % 16:
-            q = q.detach().contiguous()
+            q = q.detach().clone(memory_format=torch.contiguous_format)
             q_sb = H * D
         qp, q_st = q.data_ptr(), 0
     else:
@@ -410,7 +411,7 @@ def verify_drafts(logits, tokens, parents, uniforms, draft_logits=None, temperat
     paged_tree_decode (None: a chain), uniforms (B, n + 1) float32 in [0, 1).
     draft_logits (B, n, V): row j is the distribution the children of row j were
     drawn from; None: the tokens were picked, not drawn.  temperature: a float,
-    or a float32 (B,) tensor; 0 is greedy (the first maximum).
+    or a float32 (B,) tensor; 0 is greedy (the first maximum), above 1e30 counts as 1e30.
 
     Nodes are scanned in order, starting at row 0 with c = 0 and Z = 1.  A node
     whose parent is the current row is accepted iff u q(x) Z < p(x) - c q(x), p

@@ -122,7 +122,7 @@ def bound(y, sums, r, dtype, i8):
     (2^-18 of |q||k|, through t) and the mask's (2^-21)."""
     out = 2.0**-8 if dtype == torch.bfloat16 else 2.0**-22
     al = 2.0**-21 if dtype == torch.float32 else 2.0**-11 if i8 else 2.0**-8
-    return (out * y.norm(dim=-1) + al * sums[..., 0] + 2.0**-18 * r * sums[..., 1]
+    return (out * y.norm(dim=-1) + al * sums[..., 0] + 2.0**-18 * r.abs() * sums[..., 1]
             + 2.0**-21 * sums[..., 2] + 1e-9)
 
 

@@ -202,6 +202,84 @@ def test_nodes_past_the_table_are_not_seen(ms):
     assert y.isfinite().all() and (y[0, :2] != 0).any()
 
 
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True),
+                                      (torch.float32, False), (torch.float32, True)])
+@pytest.mark.parametrize("n", [3, 13, 20, 40])
+def test_windows_of_nothing_or_of_one_token(ms, n, dtype, q8):
+    """w <= 0 or NaN: nothing is seen, y = 0; 0 < w <= 1: the node alone."""
+    c = make(ms, 2, 6, 64, 16, 100, n, dtype, q8, n)
+    w = torch.tensor([0.0, -5.0, math.nan, 1e-40, 0.3, 1.0])
+    r = torch.full((6,), 1.2)
+    lens = torch.tensor([100, 70], dtype=torch.int32)
+    y = check(ms, c, lens, tree_parents(2, n, "random", c["g"]), r, w, dtype, q8)
+    assert (y[:, :, :3] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True),
+                                      (torch.float32, False), (torch.float32, True)])
+@pytest.mark.parametrize("n,ctas", [(2, 1), (12, 6), (30, 1)])
+def test_negative_acceptance(ms, n, ctas, dtype, q8):
+    """r < 0 prefers unlike keys, alpha up to (1 + 2 |r|)^2; one-hot V rows, whose
+    int8 scale 1 / 127 is the largest there is."""
+    c = make(ms, 2, 3, 64, 16, 150, n, dtype, q8, 3 * n)
+    if q8:
+        c["vp"].zero_()
+        c["vp"][..., 5] = 127
+        c["vs"].fill_(1.0 / 127.0)
+    lens = torch.tensor([150, 90], dtype=torch.int32)
+    check(ms, c, lens, None, torch.tensor([-1.0, -7.5, -0.2]), torch.tensor([200.0, 70.0, 33.0]), dtype, q8,
+          num_ctas=ctas)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_rows_that_start_anywhere(ms, q8):
+    """Contiguous q, k, v that do not start on 16 bytes, and size-1 dimensions of any
+    stride, are read as any other."""
+    c = make(ms, 1, 1, 64, 16, 40, 4, torch.bfloat16, q8, 8)
+    r, w = torch.full((1,), 1.2, device=DEV), torch.full((1,), 30.0, device=DEV)
+    lens = torch.full((1,), 40, dtype=torch.int32, device=DEV)
+
+    def shifted(x):
+        flat = torch.empty(x.numel() + 1, dtype=x.dtype, device=DEV)
+        flat[1:] = x.flatten().to(DEV)
+        return flat.as_strided(x.shape, (7, 64, 3, 1), 1)
+
+    rest = (lens, None, r, w, c["kp"], c["vp"], c["table"], c["ks"], c["vs"])
+    want = ms.paged_tree_decode(*(c[x].to(DEV) for x in "qkv"), *rest)
+    assert torch.equal(ms.paged_tree_decode(*(shifted(c[x]) for x in "qkv"), *rest), want)
+    held = c["kp"].clone()
+    ms.paged_append(shifted(c["k"]), shifted(c["v"]), lens, c["kp"], c["vp"], c["table"], c["ks"], c["vs"])
+    assert torch.equal(c["kp"], held)
+    if q8:
+        one = c["q"][:, 0].to(DEV)
+        moved = shifted(c["q"])[:, 0]
+        seq = lens + 1
+        tail = (seq, r, w, c["kp"], c["vp"], c["table"], c["ks"], c["vs"])
+        assert torch.equal(ms.paged_decode(one, *tail), ms.paged_decode(moved, *tail))
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.float32, True), (torch.float32, False)])
+def test_lengths_past_the_table(ms, dtype, q8):
+    """A length far past the block table reads what the table holds."""
+    c = make(ms, 2, 2, 64, 16, 60, 3, dtype, q8, 12)
+    rows = c["table"].shape[1] * 16
+    lens = torch.tensor([60, 900_000_000], dtype=torch.int32)
+    r, w = torch.full((2,), 1.2), torch.tensor([50.0, math.inf])
+    for ctas in (1, 8):
+        dev = [x.to(DEV) for x in (c["q"], c["k"], c["v"], lens)]
+        y = ms.paged_tree_decode(*dev, None, r.to(DEV), w.to(DEV), c["kp"], c["vp"], c["table"], c["ks"], c["vs"],
+                                 num_ctas=ctas)
+        assert y.isfinite().all() and (y[1, :, 0] == 0).all()    # the window lies past the table
+    prefix = tuple(None if x is None else x.cpu() for x in (c["kp"], c["vp"], c["ks"], c["vs"], c["table"]))
+    # w = inf sees every cached row (weight 1); the nodes have no rows
+    pos = list(range(rows))
+    k, v = po.cache_values(prefix[0], prefix[2], prefix[4], 1, pos), po.cache_values(prefix[1], prefix[3], prefix[4], 1, pos)
+    for i in range(3):
+        want, s = po.query(c["q"][1, i, 1], k[:, 1], v[:, 1], torch.zeros(rows), 1.2, 1.0)
+        lim = bound(want[None, None], torch.tensor(s)[None, None], r[1:], dtype, q8)
+        assert float((y[1, i, 1].double().cpu() - want).norm()) <= float(lim.max())
+
+
 @pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.float32, False), (torch.bfloat16, True)])
 @pytest.mark.parametrize("L,B,n,H,D,ps", [(1, 1, 1, 1, 16, 8), (3, 2, 5, 2, 64, 16), (2, 3, 64, 2, 128, 24)])
 def test_commit(ms, L, B, n, H, D, ps, dtype, q8):
