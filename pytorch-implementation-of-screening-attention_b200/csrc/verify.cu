@@ -68,7 +68,7 @@ __device__ __forceinline__ double exp2_64(double y) {
   return y < -1000.0 ? 0.0 : e;
 }
 
-// exp((x - m) / T) of 8 elements of a row, k = m log2(e) / T, c2 = log2(e) / T, in
+// exp((x - m) / T) of 8 elements of a row, c2 = log2(e) / T, k = c2 m, in
 // three 64-bit operations each (a chain as above ran at 1.5 exponentials per
 // cycle and SM: 64-bit FMAs of three registers at 28, conversions at 16; this
 // at 4).
@@ -76,21 +76,28 @@ __device__ __forceinline__ double exp2_64(double y) {
 // low word pair as a fixed-point number, bits 40.. its integer part n, the next 8
 // an index j, the last 32 a remainder g < 2^-8; 2^y = 2^n T[j] (1 + w) with
 // T[j] = 2^(j/256) and w = 2^g - 1 = u + u^2/2 + u^3/6, u = g ln 2, in 32 bits: the
-// dropped u^4/24 is below 3e-12, w's rounding below 2^-24 * 2.8e-3.
+// dropped u^4/24 is below 3e-12, w's rounding below 2^-24 * 2.8e-3.  Where k is
+// large (a temperature near 0) x c2 - k would lose the low bits of both, so x - m is
+// taken first, with one operation more.
 constexpr int kTab = 256;
 __device__ __forceinline__ void fill_table(double* tab) {
   for (int i = threadIdx.x; i < kTab; i += blockDim.x) tab[i] = 2.0 * exp2_64((double)i / kTab - 1.0);
 }
-__device__ __forceinline__ void exp8(const float (&x)[8], double c2, double k, const double* tab,
+__device__ __forceinline__ void exp8(const float (&x)[8], double c2, double m, const double* tab,
                                      double (&o)[8]) {
   // step by step over the eight, so that their chains run side by side (one
   // after another took 1170 cycles a warp, this 450)
-  const double base = 6144.0 - k;
+  const double k = c2 * m, base = 6144.0 - k;
   double t[8], w[8];
   int hi[8];
   float u[8];
+  if (fabs(k) <= 8192.0) {           // uniform
 #pragma unroll
-  for (int e = 0; e < 8; ++e) t[e] = fma(c2, wide(x[e]), base);
+    for (int e = 0; e < 8; ++e) t[e] = fma(c2, wide(x[e]), base);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = fma(c2, wide(x[e]) - m, 6144.0);
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     hi[e] = __double2hiint(t[e]);
@@ -175,7 +182,7 @@ __device__ __forceinline__ Part part_of(int V, int rank, int C) {
 template <typename T>
 struct Weights {
   const T *p, *q;
-  double kp, kq, ip, iq;
+  double mp, mq, ip, iq;   // maxima; factors
   int n_gone;
   const int* gone;
 };
@@ -185,10 +192,10 @@ __device__ __forceinline__ void weights8(const Weights<T>& w, double c2, const d
   float x[8], y[8];
   load8<T, VEC>(w.p, v, V, x);
   if (w.q) load8<T, VEC>(w.q, v, V, y);
-  exp8(x, c2, w.kp, tab, o);
+  exp8(x, c2, w.mp, tab, o);
   if (w.q) {
     double f[8];
-    exp8(y, c2, w.kq, tab, f);
+    exp8(y, c2, w.mq, tab, f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = fmax(w.ip * o[e] - w.iq * f[e], 0.0);
   }
@@ -286,7 +293,7 @@ __device__ RowSum row_part(const T* row, const Part& t, int V, double c2, const 
                            double* wsum) {
   RowSum r = top_part<T, VEC>(row, t, V, sh);
   if (r.m != -INFINITY) {            // uniform
-    const Weights<T> w{row, nullptr, c2 * wide(r.m), 0.0, 0.0, 0.0, 0, nullptr};
+    const Weights<T> w{row, nullptr, wide(r.m), 0.0, 0.0, 0.0, 0, nullptr};
     r.s += sum_part<T, VEC>(w, c2, tab, t, V, wsum);
   }
   return r;
@@ -296,9 +303,10 @@ __device__ __forceinline__ float temp_of(const screen_verify_args& a, int b) {
   return a.temperatures ? a.temperatures[b] : a.temperature;
 }
 // log2(e) / T; T not above 0 means the maximum only (any positive T then tells
-// whether the row is usable)
+// whether the row is usable).  T counts as 1e30 above that: -inf, held as -2^128,
+// keeps the weight 0.
 __device__ __forceinline__ double scale_of(float temp) {
-  return 1.4426950408889634 / (temp > 0.f ? (double)temp : 1.0);
+  return 1.4426950408889634 / (temp > 0.f ? fmin((double)temp, 1e30) : 1.0);
 }
 
 // ---------------------------------------------------------------------------
@@ -534,7 +542,7 @@ __global__ void __launch_bounds__(kT, 2) walk_kernel(screen_verify_args a, const
     w.rows(cur, prow, qrow, P, Q, before, mine);
     if (!usable(P)) break;                        // no distribution: no token
     if (qrow && !usable(Q)) left = 0;             // nothing was drawn from this
-    const double kp = w.c2 * wide(P.m), kq = w.c2 * wide(Q.m);
+    const double mp = wide(P.m), mq = wide(Q.m);
     double c = 0.0, z = 1.0, all = P.s, out_mass = 0.0;
     int n_gone = 0, next = -1;
     bool stale = given != nullptr;                // all and wsum are not the residual's
@@ -549,8 +557,8 @@ __global__ void __launch_bounds__(kT, 2) walk_kernel(screen_verify_args a, const
         px = x == P.arg ? 1.0 : 0.0;
         qx = !drawn || x == Q.arg ? 1.0 : 0.0;
       } else {
-        px = exp2_64(fma(w.c2, wide(lp[i]), -kp)) / P.s;
-        qx = drawn ? exp2_64(fma(w.c2, wide(lq[i]), -kq)) / Q.s : 1.0;
+        px = exp2_64(w.c2 * (wide(lp[i]) - mp)) / P.s;
+        qx = drawn ? exp2_64(w.c2 * (wide(lq[i]) - mq)) / Q.s : 1.0;
       }
       if (dup) px = 0.0;
       const double rest = px - c * qx;
@@ -564,7 +572,7 @@ __global__ void __launch_bounds__(kT, 2) walk_kernel(screen_verify_args a, const
         if (greedy) {                             // p and q are one point each
           z = fmax(P.arg == Q.arg ? 1.0 - c : 1.0, 0.0);
         } else {
-          z = all = w.sum({prow, qrow, kp, kq, 1.0 / P.s, c / Q.s, 0, gone}, before, mine);
+          z = all = w.sum({prow, qrow, mp, mq, 1.0 / P.s, c / Q.s, 0, gone}, before, mine);
           stale = false;
         }
       } else if (!dup) {
@@ -579,7 +587,7 @@ __global__ void __launch_bounds__(kT, 2) walk_kernel(screen_verify_args a, const
           out_mass += px;
           z = 1.0 - out_mass;
           if (z < 1e-6) {                         // too little left for a difference
-            all = w.sum({prow, nullptr, kp, 0.0, 0.0, 0.0, n_gone, gone}, before, mine);
+            all = w.sum({prow, nullptr, mp, 0.0, 0.0, 0.0, n_gone, gone}, before, mine);
             z = all / P.s;
             stale = false;
           }
@@ -598,7 +606,7 @@ __global__ void __launch_bounds__(kT, 2) walk_kernel(screen_verify_args a, const
       break;
     }
     const double u = a.uniforms[(long long)b * a.u_sb + n];
-    Weights<T> wt{prow, nullptr, kp, kq, 0.0, 0.0, n_gone, gone};
+    Weights<T> wt{prow, nullptr, mp, mq, 0.0, 0.0, n_gone, gone};
     if (c > 0.0) {
       wt.q = qrow;
       wt.ip = 1.0 / P.s;

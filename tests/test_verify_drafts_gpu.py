@@ -181,3 +181,25 @@ def test_captured(ms):
         g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("B,V", [(2, 501), (40, 50257)])
+def test_temperatures_near_zero_and_huge(ms, B, V, drawn, dtype):
+    """Temperatures down to the smallest float: ties of the maximum share the
+    probability; up to 1e30: -inf entries keep probability 0."""
+    for i, temp in enumerate((2.0**-12, 2.0**-20, 2.0**-60, 2.0**-140, 2.0**99)):
+        c = case(B, 3, V, "chain", drawn, 1.0, dtype, 50 + i)
+        top = c["logits"].float().max(-1, keepdim=True).values
+        for at in (3, 77, V - 2):                                # three of the maximum
+            c["logits"][..., at] = top[..., 0].to(dtype)
+        c["logits"][:, :, 9] = -math.inf
+        c["tokens"][:, 0] = 77
+        check(ms, c, temp)
+
+
+@pytest.mark.parametrize("tiny", [1e-45, 1e-30])
+def test_tiny_temperatures_per_sequence(ms, tiny):
+    c = case(3, 2, 301, "chain", True, 1.0, torch.float32, 9)
+    check(ms, c, torch.tensor([tiny, 1.0, 0.0]).to(DEV))
