@@ -334,7 +334,9 @@ class MultiscreenLM(nn.Module):
         tokens, rows = [last], []
         for i in range(num_draft + 1):
             # the last draft's step only leaves its row in the drafting cache
-            lg = draft.decode_step(tokens[-1], lens + i, caches[1], states[1], clamp_position=True)
+            # (a row without a distribution, with a NaN say, yields token -1)
+            lg = draft.decode_step(tokens[-1].clamp_min(0), lens + i, caches[1], states[1],
+                                   clamp_position=True)
             if i < num_draft:
                 lg = _keep_top(lg, top_k)
                 rows.append(lg)
@@ -343,8 +345,11 @@ class MultiscreenLM(nn.Module):
                 tokens.append(drawn)
         chain = torch.cat(tokens, 1)
         logits = _keep_top(self.tree_step(chain, lens, caches[0], state=states[0]), top_k)
+        rows = torch.stack(rows, 1)
+        if rows.dtype is not logits.dtype:     # the drafts were drawn from the rows as they are
+            rows, logits = rows.float(), logits.float()
         out, _, counts = verify_drafts(logits, chain[:, 1:], None, uniforms[:, num_draft:],
-                                       draft_logits=torch.stack(rows, 1).to(logits.dtype),
+                                       draft_logits=rows,
                                        temperature=temperature)
         return out, counts
 

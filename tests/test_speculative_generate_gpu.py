@@ -181,3 +181,39 @@ def test_speculative_samples_follow_the_model(ms):
     ok = want > 0
     assert seen[~ok].sum() == 0
     assert float(((seen - want)[ok] ** 2 / want[ok]).sum()) < 24.3
+
+
+@pytest.mark.parametrize("graph", [True, False])
+def test_rows_without_a_distribution_yield_minus_one(ms, graph):
+    """A model whose logits are NaN: the tokens say so, nothing is looked up with
+    them; with a drafting model of that kind the tokens are the model's own."""
+    m, d = lm(ms, torch.float32), lm(ms, torch.float32, layers=1)
+    ids = torch.randint(0, 97, (2, 17), device=DEV)
+    want = m.generate(ids, 9, top_k=1)
+    with torch.no_grad():
+        d.norm.weight.fill_(float("nan"))
+    assert torch.equal(m.generate_speculative(ids, d, 9, num_draft=3, temperature=0.0, cuda_graph=graph), want)
+    out = d.generate_speculative(ids, m, 9, num_draft=3, cuda_graph=graph)
+    assert torch.equal(out[:, :17], ids) and (out[:, 17:] == -1).all()
+
+
+def test_drafts_are_verified_against_the_rows_they_were_drawn_from(ms, monkeypatch):
+    """An fp32 drafting model under a bf16 model: its rows are not rounded."""
+    m, d = lm(ms, torch.bfloat16), lm(ms, torch.float32, layers=1)
+    ids = torch.randint(0, 97, (2, 17), device=DEV)
+    seen = []
+    import sys
+    mod = sys.modules[type(m).__module__]
+    real = mod.verify_drafts
+
+    def spy(logits, *args, **kw):
+        seen.append((logits, kw.get("draft_logits")))
+        return real(logits, *args, **kw)
+
+    monkeypatch.setattr(mod, "verify_drafts", spy)
+    out = m.generate_speculative(ids, d, 4, num_draft=2, cuda_graph=False)
+    assert out.shape == (2, 21) and int(out.min()) >= 0
+    drawn = [x for x, rows in seen[1:] if rows is None][:2]
+    logits, rows = next((x, r) for x, r in seen if r is not None)
+    assert logits.dtype == rows.dtype == torch.float32
+    assert torch.equal(torch.cat(drawn, 1), rows)
