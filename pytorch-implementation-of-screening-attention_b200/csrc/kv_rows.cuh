@@ -60,9 +60,10 @@ __device__ __forceinline__ void load8f(const T* p, float (&x)[8]) {
 //   m = round_half_even(127 x / max|x|),  scale = 1 / max(|m|, 127 eps / max|x|),
 // so scale * m is the unit form of the rounded raw row.  The integers do not
 // depend on any order of summation: max|x| is exact, and |m|^2 <= 128 * 127^2 is
-// summed in integers.  For bf16 values (BF) 127 x is exact in 32 bits and the
-// quotient correctly rounded (a product with the rounded reciprocal and one
-// remainder step), which no half can cross; for fp32 a quotient so near a half
+// summed in integers.  For bf16 values (BF) 127 x is exact in 32 bits, and a product
+// with the approximate reciprocal and one remainder step leave the quotient right
+// to 2^-24 (its nearest float, but for 2^-44 of it): a half comes out exactly, and
+// no other quotient of 8-bit significands lies within 2^-17 of one; for fp32 a quotient so near a half
 // that 32 bits cannot tell (127 * 2^-23 at most; one in 16,000) is decided by an
 // exact comparison in 64 bits.  A row with an infinity or NaN becomes m = 0, scale
 // NaN.
@@ -70,6 +71,7 @@ struct Int8Scale {
   float up, am, inv;     // x is scaled by up (0: a row of zeros); am = max|up x|
 };
 // of a row whose largest magnitude has the bits `top`
+template <bool BF>
 __device__ __forceinline__ Int8Scale int8_scale(uint32_t top) {
   const bool finite = top < 0x7f800000u;
   const float amax = __uint_as_float(top);
@@ -80,7 +82,8 @@ __device__ __forceinline__ Int8Scale int8_scale(uint32_t top) {
     s.up = finite && top ? (amax < 1.0f ? 0x1p100f : 0x1p-100f) : 0.f;
     s.am = s.up != 0.f ? amax * s.up : 1.0f;
   }
-  s.inv = 1.0f / s.am;
+  if constexpr (BF) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.inv) : "f"(s.am));
+  else s.inv = 1.0f / s.am;
   return s;
 }
 // E elements as int8, four to a word, and the sum of their squares added to ss.
@@ -93,10 +96,23 @@ __device__ __forceinline__ void int8_pack(float (&x)[E], const Int8Scale& s, uin
   const float magic = 12582912.0f;   // 1.5 * 2^23: rounds to an integer in the low byte
   float f[E];
   if constexpr (BF) {
+    // two elements an instruction, step by step over the row's part
+    const float2 c127 = make_float2(127.0f, 127.0f), inv = make_float2(s.inv, s.inv);
+    const float2 neg = make_float2(-s.am, -s.am), mg = make_float2(magic, magic);
+    float2 d[E / 2], q[E / 2];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float d = 127.0f * x[e], q = d * s.inv;
-      f[e] = fmaf(fmaf(-q, s.am, d), s.inv, q) + magic;
+    for (int e = 0; e < E / 2; ++e) d[e] = __fmul2_rn(make_float2(x[2 * e], x[2 * e + 1]), c127);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) q[e] = __fmul2_rn(d[e], inv);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) d[e] = __ffma2_rn(q[e], neg, d[e]);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) q[e] = __ffma2_rn(d[e], inv, q[e]);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      q[e] = __fadd2_rn(q[e], mg);
+      f[2 * e] = q[e].x;
+      f[2 * e + 1] = q[e].y;
     }
   } else {
     bool near = false;
@@ -136,21 +152,4 @@ __device__ __forceinline__ float int8_stored_scale(uint32_t top, int ss, float e
   if (!(amax >= eps)) scale = top ? fminf(scale, amax / (127.0f * eps)) : 0.f;
   return top < 0x7f800000u ? scale : __uint_as_float(0x7fc00000u);
 }
-// A row held by a group of G lanes, E elements a lane.  All 32 lanes of the warp
-// must call it; x is used up.
-template <int G, int E, bool BF>
-__device__ __forceinline__ void int8_row(float (&x)[E], float eps, uint32_t (&m)[E / 4],
-                                         float& scale) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o, G));
-  int ss = 0;
-  int8_pack<E, BF>(x, int8_scale(top), m, ss);
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
-  scale = int8_stored_scale(top, ss, eps);
-}
-
 }  // namespace screen

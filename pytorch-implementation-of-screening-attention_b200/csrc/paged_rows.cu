@@ -34,12 +34,30 @@ __device__ __forceinline__ RowBlock row_block(int B, int H, int n, int tokens) {
   return r;
 }
 // ---------------------------------------------------------------------------
-// Append to int8 pages.  Bound by HBM: D * sizeof(T) bytes in, D + 4 out per
-// row.
+// Append to int8 pages.  D * sizeof(T) bytes in, D + 4 out per row; bound by issue
+// before HBM, so two elements go through an instruction where one takes pairs,
+// and a token's place in the pages is looked up once for all its heads.
 // ---------------------------------------------------------------------------
+// The bits of the largest magnitude among the row whose 16-byte parts G lanes hold.
+template <typename T, int G>
+__device__ __forceinline__ uint32_t row_top(const uint4& u) {
+  uint32_t top;
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t abs = 0x7fff7fffu;
+    top = __vmaxu2(__vmaxu2(u.x & abs, u.y & abs), __vmaxu2(u.z & abs, u.w & abs));
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o, G));
+    return max(top & 0xffff0000u, top << 16);
+  } else {
+    const uint32_t abs = 0x7fffffffu;
+    top = max(max(u.x & abs, u.y & abs), max(u.z & abs, u.w & abs));
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o, G));
+    return top;
+  }
+}
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, float (&x)[16 / sizeof(T)]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void widen(const uint4& u, float (&x)[16 / sizeof(T)]) {
   if constexpr (sizeof(T) == 2) {
     const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), d = unpack_bf16(u.w);
     x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
@@ -52,43 +70,52 @@ __device__ __forceinline__ void load16(const T* p, float (&x)[16 / sizeof(T)]) {
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(kThreads) append8_kernel(screen_paged_append_args a, int tokens,
                                                                 unsigned inv_heads) {
+  constexpr int E = 16 / (int)sizeof(T), G = D / E, GROUPS = kThreads / G;
+  __shared__ long long base[R * GROUPS];   // row of head 0 per token of the block, -1 none
   pdl_wait();
   pdl_trigger();
-  constexpr int E = 16 / (int)sizeof(T), G = D / E, GROUPS = kThreads / G;
   const RowBlock rb = row_block(a.B, a.H, a.n_new, tokens);
   const int gl = threadIdx.x % G, grp = threadIdx.x / G;
   const long long sb = rb.isv ? a.v_sb : a.k_sb, st = rb.isv ? a.v_st : a.k_st;
-  const T* src = reinterpret_cast<const T*>(rb.isv ? a.v : a.k) + (long long)rb.b * sb + gl * E;
+  const T* src = reinterpret_cast<const T*>(rb.isv ? a.v : a.k) + (long long)rb.b * sb + rb.n0 * st + gl * E;
   const int* table = a.cache.block_table + (long long)rb.b * a.cache.max_blocks;
-  const long long pos0 = a.positions[rb.b];
-  signed char* pages = reinterpret_cast<signed char*>(rb.isv ? a.cache.v_pages : a.cache.k_pages);
+  const long long pos0 = (long long)a.positions[rb.b] + rb.n0;
+  signed char* pages = reinterpret_cast<signed char*>(rb.isv ? a.cache.v_pages : a.cache.k_pages) + gl * E;
   float* scales = rb.isv ? a.v_scales : a.k_scales;
+  for (int t = threadIdx.x; t < tokens; t += kThreads) base[t] = table_row(a.cache, table, a.H, 0, pos0 + t);
 #pragma unroll 1
   for (int r0 = 0; r0 < rb.rows; r0 += R * GROUPS) {   // uniform: the shuffles need every lane
-    float x[R][E];
-    long long row[R];
+    uint4 u[R];
+    int t[R], h[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int r = r0 + i * GROUPS + grp;
-      row[i] = -1;
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+      u[i] = make_uint4(0u, 0u, 0u, 0u);
+      t[i] = -1;
       if (r < rb.rows) {
-        const int t = div_heads(r, a.H, inv_heads), h = r - t * a.H, n = rb.n0 + t;
-        load16(src + n * st + (long long)h * D, x[i]);
-        row[i] = table_row(a.cache, table, a.H, h, pos0 + n);
+        t[i] = div_heads(r, a.H, inv_heads);
+        h[i] = r - t[i] * a.H;
+        u[i] = *reinterpret_cast<const uint4*>(src + t[i] * st + h[i] * D);
       }
     }
+    if (r0 == 0) __syncthreads();
 #pragma unroll
     for (int i = 0; i < R; ++i) {
+      float x[E];
       uint32_t m[E / 4];
-      float sc;
-      int8_row<G, E, sizeof(T) == 2>(x[i], a.eps, m, sc);
-      if (row[i] >= 0) {
-        signed char* dst = pages + row[i] * D + gl * E;
+      const uint32_t top = row_top<T, G>(u[i]);
+      widen<T>(u[i], x);
+      int ss = 0;
+      int8_pack<E, sizeof(T) == 2>(x, int8_scale<sizeof(T) == 2>(top), m, ss);
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
+      long long row = t[i] < 0 ? -1 : base[t[i]];
+      if (row >= 0) {
+        row += (long long)h[i] * a.cache.page_size;
+        signed char* dst = pages + row * D;
         if constexpr (E == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(m[0], m[1]);
         else *reinterpret_cast<uint32_t*>(dst) = m[0];
-        if (gl == 0) scales[row[i]] = sc;
+        if (gl == 0) scales[row] = int8_stored_scale(top, ss, a.eps);
       }
     }
   }

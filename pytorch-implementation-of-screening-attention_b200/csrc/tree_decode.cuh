@@ -277,7 +277,7 @@ __device__ __forceinline__ void append_rows(const screen_tree_args& a, const Nod
         for (int j = 0; j < C; ++j) tops[k] = max(tops[k], __float_as_uint(mine[j].x));
         uint32_t m[2];
         ss[k] = 0;
-        int8_pack<N, sizeof(TA) == 2>(x[k], int8_scale(tops[k]), m, ss[k]);
+        int8_pack<N, sizeof(TA) == 2>(x[k], int8_scale<sizeof(TA) == 2>(tops[k]), m, ss[k]);
         if (row[k] >= 0) *reinterpret_cast<uint2*>(dst) = make_uint2(m[0], m[1]);
       } else {
         float p[2 * C];

@@ -171,3 +171,24 @@ def test_decode_empty_places(ms):
     assert y2[1, 0].isfinite().all() and torch.equal(y2[3], y[3])
     near = ms.paged_decode(q.to(DEV), lens, r, torch.full((H,), 3.0, device=DEV), kp, vp, table, ks, vs)
     assert near[1, 1].isfinite().all()            # the window ends before it
+
+
+def test_every_bf16_quotient(ms):
+    """All pairs of 8-bit significands, eight binades down: the integers are those
+    of the exact quotient, halves to even."""
+    A = torch.arange(128, 256).repeat_interleave(8)                     # a row's largest value
+    X = torch.arange(128, 256)
+    shift = torch.arange(8).repeat(128)
+    rows = (X[None] * 2.0 ** -shift[:, None].float()).clamp(max=A[:, None].float())
+    rows[:, 5] = A.float()
+    rows[:, ::3] *= -1
+    k = rows.view(1, 1024, 1, 128).to(torch.bfloat16)
+    assert torch.equal(k.float().view(1024, 128), rows)
+    kp, vp, table, ks, vs = empty_cache(1, 1, 128, 64, 16)
+    ms.paged_append(k.to(DEV), (k * 2.0**-60).to(DEV), torch.zeros(1, dtype=torch.int32, device=DEV), kp, vp, table, ks, vs)
+    # 127 |x| / A = n / A' in integers, rounded half to even
+    num, den = (127 * rows.abs() * 2.0**shift[:, None].float()).long(), (A << shift)[:, None]
+    q, rest = num // den, num % den
+    want = (q + ((2 * rest > den) | ((2 * rest == den) & (q % 2 == 1))).long()) * rows.sign().long()
+    for pages in (kp, vp):
+        assert torch.equal(pages[table[0].long()].cpu().view(1024, 128).long(), want)
