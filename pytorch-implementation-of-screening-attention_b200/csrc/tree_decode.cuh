@@ -90,8 +90,12 @@ __device__ __forceinline__ bool find_run(const TreeParams& p, int* tiles, SegSlo
   __shared__ int run_s[2];
   const int ctas = gridDim.x;
   long long sum = 0;
+  // writing the nodes' rows takes the time of about a tile per 16 of them, behind a
+  // segment's last (counted so, 64 nodes over 32K keys: 136 us, not counted 142)
+  const int extra = p.a.k ? (p.a.n + 15) / 16 : 0;
   for (int j = tid; j < segs; j += kThreads) {
-    const int nt = tree_range(p, j / p.a.H, j % p.a.H).nt;
+    const Range rg = tree_range(p, j / p.a.H, j % p.a.H);
+    const int nt = rg.nt + (rg.any ? extra : 0);
     tiles[j] = nt;
     sum += nt;
   }
@@ -158,7 +162,7 @@ __device__ __forceinline__ bool find_run(const TreeParams& p, int* tiles, SegSlo
   __syncthreads();                   // `tiles` has been read
   g = tree_range(p, seg / p.a.H, seg % p.a.H);
   c0 = g.t0 + (int)((long long)nt * i / n);
-  c1 = g.t0 + (int)((long long)nt * (i + 1) / n) - 1;
+  c1 = min(g.t0 + (int)((long long)nt * (i + 1) / n), g.t0 + g.nt) - 1;   // a run may be empty
   whole = n == 1;
   if (i == 0 && tid == 0) slots[seg] = SegSlots{(int)blockIdx.x, whole ? 0 : n};
   return true;
@@ -336,6 +340,18 @@ __device__ __forceinline__ void store_row(const screen_tree_args& a, int b, int 
 #pragma unroll
   for (int e = 0; e < PER; ++e)
     if (lane + 32 * e < D) y[lane + 32 * e] = from_f<TA>(present ? o[e] * g : 0.f);
+}
+
+// The whole of an SM's L1 as shared memory for `fn`: an SM whose split was made for
+// another kernel's CTAs takes fewer of this one's until it has run empty.
+inline void prefer_shared(const void* fn) {
+  static std::mutex mu;
+  static std::set<std::pair<int, const void*>> done;
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) return;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!done.insert({dev, fn}).second) return;
+  cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
 }
 
 // One CTA per segment, or at most as many as are resident at once (a CTA per segment

@@ -170,11 +170,13 @@ void launch_f32(const TreeParams& p, float* part, cudaStream_t s) {
   if (smem < kMaxShared * 4) smem = kMaxShared * 4;   // find_run
   constexpr int kMost = (kMaxN * D + 2 * kKeys * (D + 4) + kMaxN * 33) * 4;
   if (ensure_smem_optin((const void*)tree_f32_kernel<D>, kMost) != cudaSuccess) return;
+  prefer_shared((const void*)tree_f32_kernel<D>);
   launch_pdl(tree_f32_kernel<D>, tree_grid(p, 3), dim3(kThreads), smem, s, p, part);
 }
 template <typename TA, int D>
 void launch_finish(const TreeParams& p, const float* part, cudaStream_t s) {
   const long long rows = (long long)p.a.B * p.a.H * p.a.n;
+  prefer_shared((const void*)tree_finish_kernel<TA, D>);
   launch_pdl(tree_finish_kernel<TA, D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, p, part);
 }
 template <typename TA>

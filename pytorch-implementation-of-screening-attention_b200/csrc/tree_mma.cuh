@@ -99,7 +99,10 @@ struct Cfg {
   static_assert(SMEM >= kAppendScratch && SMEM >= kMaxShared * 4, "append_rows and find_run work in it");
   // CTAs per SM the registers are cut to: what a thread holds of O and q decides
   static constexpr int HELD = D_ / 2 + D_ / 4 * (QHL ? 2 : 1);
-  static constexpr int MINB = HELD <= 32 ? 4 : HELD <= 64 ? 3 : 2;
+  // (a group of four warps on int8 pages waits at its barriers and gains by a fourth
+  // CTA: 64 nodes over 32K keys 142 us, 148 with three)
+  static constexpr int MINB =
+      HELD <= 32 ? 4 : HELD <= 64 ? (CONV && MG_ == 4 && !QHL ? 4 : 3) : 2;
 };
 
 // Byte offset of 16-byte chunk c of row r in a tile: the XOR makes the fragment
@@ -322,17 +325,24 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
   // --- a stage: KT keys, their addresses and facts ---------------------------
   const int s0 = c0 * (kTile / KT), s1 = (c1 + 1) * (kTile / KT) - 1;
   const int* table = a.cache.block_table + (long long)b * a.cache.max_blocks;
-  // row of this lane's key of stage x, -1 none
-  auto key_row = [&](int x) -> long long {
+  // page of this lane's key of stage x (-1 none) and the key's place in it; the row,
+  // -1 none, is made of them as late as it is needed, so that nothing waits for
+  // the table
+  struct Key {
+    int page;
+    unsigned at;
+  };
+  auto key_page = [&](int x) -> Key {
     const long long pos = (long long)x * KT + lane;
-    if (lane >= KT || x > s1 || pos < rg.first || pos >= lens + a.n) return -1;
-    if (pos >= lens && !nodes.line[pos - lens]) return -1;
+    if (lane >= KT || x > s1 || pos < rg.first || pos >= lens + a.n) return Key{-1, 0};
+    if (pos >= lens && !nodes.line[pos - lens]) return Key{-1, 0};
     const unsigned q = (unsigned)pos;                // a table holds < 2^31 positions
     const unsigned blk = ps_shift >= 0 ? q >> ps_shift : q / (unsigned)ps;
-    if (blk >= (unsigned)a.cache.max_blocks) return -1;
-    const int page = table[blk];
-    if (page < 0 || page >= a.cache.num_pages) return -1;
-    return ((long long)page * a.H + h) * ps + (q - blk * (unsigned)ps);
+    if (blk >= (unsigned)a.cache.max_blocks) return Key{-1, 0};
+    return Key{table[blk], q - blk * (unsigned)ps};
+  };
+  auto key_row = [&](Key k) -> long long {
+    return (unsigned)k.page < (unsigned)a.cache.num_pages ? ((long long)k.page * a.H + h) * ps + k.at : -1;
   };
   // In a group of several warps they take turns in looking a stage's rows up: its
   // warp leaves them in a plan (rows, then the first row if all follow it, else
@@ -448,17 +458,18 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
   };
 
   // --- the first stages, under way while the queries are brought in ------------
-  auto start = [&]() -> long long {
+  auto start = [&]() -> Key {
     // the group's stage number `turn` sits in ring slot turn % S
-    long long rows[S];
+    Key keys[S];
 #pragma unroll
-    for (int i = 0; i < S; ++i) rows[i] = key_row(s0 + wk + i * C::WK);
+    for (int i = 0; i < S; ++i) keys[i] = key_page(s0 + wk + i * C::WK);
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) load_stage(i, i, rows[i], false);
-    if (C::MG > 1 && mg == (S - 1) % C::MG) make_plan(S - 1, rows[S - 1]);
-    return rows[S - 1];
+    for (int i = 0; i < S - 1; ++i) load_stage(i, i, key_row(keys[i]), false);
+    if (C::MG > 1 && mg == (S - 1) % C::MG) make_plan(S - 1, key_row(keys[S - 1]));
+    return keys[S - 1];
   };
-  long long next = rg.any ? start() : -1;
+  Key next{-1, 0};
+  if (rg.any) next = start();
 
   // --- queries: fragments, per-row factors ------------------------------------
   uint32_t qa[C::KS][4];
@@ -575,10 +586,10 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
       for (int x = s0 + wk, turn = 0; x <= s1; x += C::WK, ++turn) {
         cp_async_wait<S - 2 - AHEAD>();
         group_sync();
-        load_stage(turn + S - 1, fill, next, true);
+        load_stage(turn + S - 1, fill, key_row(next), true);
         if (C::MG == 1 || mg == (turn + S) % C::MG) {
-          next = key_row(x + S * C::WK);
-          if constexpr (C::MG > 1) make_plan(turn + S, next);
+          next = key_page(x + S * C::WK);
+          if constexpr (C::MG > 1) make_plan(turn + S, key_row(next));
         }
         const unsigned char* st = ring + (size_t)slot * C::STAGE_B;
         const float* cs = reinterpret_cast<const float*>(st + 2 * C::TILE_B);
@@ -867,6 +878,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
 template <class C>
 void launch_tree(const TreeParams& p, float* ws, cudaStream_t s) {
   if (ensure_smem_optin((const void*)tree_mma_kernel<C>, C::SMEM) != cudaSuccess) return;
+  prefer_shared((const void*)tree_mma_kernel<C>);
   launch_pdl(tree_mma_kernel<C>, tree_grid(p, C::MINB), dim3(kThreads), (size_t)C::SMEM, s, p, ws);
 }
 // A warp for every 16 queries; up to 8 queries the lower half of a tile is not

@@ -356,3 +356,14 @@ def test_captured_and_on_two_streams(ms, q8):
     for o, x in zip(outs, want):
         assert torch.equal(o, x)
     assert torch.equal(eager, want[0])
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)])
+@pytest.mark.parametrize("n", [1, 33, 64])
+@pytest.mark.parametrize("T", [0, 3, 63, 250])
+def test_runs_shorter_than_a_tree(ms, dtype, q8, n, T):
+    """More CTAs than tiles: runs of one tile, of the nodes' rows alone, of nothing."""
+    c = make(ms, 2, 2, 64, 16, T, n, dtype, q8, n + T)
+    lens = torch.tensor([T, max(0, T - 9)], dtype=torch.int32)
+    r, w = torch.tensor([1.1, 1.4]), torch.tensor([400.0, 20.0])
+    check(ms, c, lens, tree_parents(2, n, "random", c["g"]), r, w, dtype, q8, num_ctas=592)
