@@ -2,6 +2,7 @@
 // or int8 pages with bf16 / fp32 activations.
 #pragma once
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "tree_decode.cuh"
 
 namespace screen {
@@ -491,7 +492,9 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
     const TA* q = reinterpret_cast<const TA*>(a.q) + (long long)b * a.q_sb + (long long)i * a.q_st +
                   (long long)h * D;
     float x[C::KS][4];
-    float ss = 0.f;
+    // QHL: an error of |q| is one of every score, r / t times over in alpha: 64 bits
+    using Sum = typename std::conditional<C::QHL, double, float>::type;
+    Sum ss = 0;
     uint32_t top = 0;
 #pragma unroll
     for (int s = 0; s < C::KS; ++s)
@@ -514,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
     for (int s = 0; s < C::KS; ++s)
 #pragma unroll
       for (int f = 0; f < 4; ++f) {
-        ss = fmaf(x[s][f], x[s][f], ss);
+        ss = fma((Sum)x[s][f], (Sum)x[s][f], ss);
         top = max(top, __float_as_uint(x[s][f]) & 0x7fffffffu);
       }
     ss += __shfl_xor_sync(0xffffffffu, ss, 1);
@@ -549,8 +552,9 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
           qa[s][2 * f + e] = pack_bf16(x[s][2 * f], x[s][2 * f + 1]);
         }
       }
-    // S = q.k scale / max(|q|, eps), times r; scale first: 2^ex / |q| <= 1
-    rq[e] = r / up * (scale / fmaxf(sqrtf(ss), a.eps));
+    // S = q.k scale / max(|q|, eps), times r; scale first: 2^ex / |q| <= 1.  QHL: -S
+    if constexpr (C::QHL) rq[e] = (float)(-(double)scale / fmax(sqrt(ss), (double)a.eps));
+    else rq[e] = r / up * (scale / fmaxf(sqrtf(ss), a.eps));
     const bool live = in && nodes.line[i] != 0;
     dep[e] = live ? nodes.depth[i] : 0;
     float sn, cn;
@@ -561,7 +565,8 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
     si[e] = (C::I8 ? 0x1p19f : 0.5f) * sn;
     if (!live) rq[e] = __uint_as_float(0x7fc00000u);  // t = NaN: sees nothing
   }
-  const float2 one_r = both((1.0f - r) / up);
+  // t = r S + (1 - r); QHL: 1 - r (1 - S), whose roundings do not grow with r
+  const float2 one_r = both((1.0f - r) / up), nr = both(-r / up), one = both(1.0f / up);
 
   float o[C::NT][4];
   // pass 0 takes every V row and scale as finite.  A non-finite one times
@@ -608,27 +613,36 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
         constexpr int N8 = 2 * C::NK;
         float2 s[N8][RH];                            // keys 2t, 2t + 1 of an 8-key tile
         {
-          float c[N8][4], d[C::QHL ? N8 : 1][4];
+          float c[N8][4];
+          // QHL: the tensor core's sums truncate, so a k step's products are summed
+          // from zero, the small ones first, and the steps in fp32 (y over 11K keys is
+          // 0.7e-6 off; 1.0e-6 with one chain, |q| in 32 bits and t = r S + (1 - r))
+          auto score_hl = [&](float (&c)[N8][4], int x2, const uint32_t (&k2)[N8][2]) {
+            float d[N8][4];
+#pragma unroll
+            for (int nt = 0; nt < N8; ++nt) mma_first<true>(d[nt], ql[x2], k2[nt][0], k2[nt][1]);
+#pragma unroll
+            for (int nt = 0; nt < N8; ++nt) mma_f16(d[nt], qa[x2], k2[nt][0], k2[nt][1]);
+#pragma unroll
+            for (int nt = 0; nt < N8; ++nt)
+#pragma unroll
+              for (int f = 0; f < 2 * RH; ++f) c[nt][f] = x2 == 0 ? d[nt][f] : c[nt][f] + d[nt][f];
+          };
           if constexpr (C::LDM) {
 #pragma unroll
             for (int x2 = 0; x2 < C::KS; ++x2) {
               uint32_t kb[N8][2];
 #pragma unroll
               for (int kg = 0; kg < C::NK; ++kg) load_k16<C>(kt, kg * 16, x2, lane, kb[2 * kg], kb[2 * kg + 1]);
-              // QHL: the small products first, and apart: the tensor core's sums
-              // truncate
               if constexpr (C::QHL) {
+                score_hl(c, x2, kb);
+              } else {
 #pragma unroll
                 for (int nt = 0; nt < N8; ++nt) {
-                  if (x2 == 0) mma_first<true>(d[nt], ql[x2], kb[nt][0], kb[nt][1]);
-                  else mma_f16(d[nt], ql[x2], kb[nt][0], kb[nt][1]);
+                  if (x2 == 0) mma_first<C::I8>(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
+                  else if constexpr (C::I8) mma_f16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
+                  else mma_b16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
                 }
-              }
-#pragma unroll
-              for (int nt = 0; nt < N8; ++nt) {
-                if (x2 == 0) mma_first<C::I8>(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
-                else if constexpr (C::I8) mma_f16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
-                else mma_b16(c[nt], qa[x2], kb[nt][0], kb[nt][1]);
               }
             }
           } else {
@@ -638,26 +652,22 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
 #pragma unroll
             for (int x2 = 0; x2 < C::KS; ++x2) {
               if constexpr (C::QHL) {
+                uint32_t k2[N8][2];
+#pragma unroll
+                for (int nt = 0; nt < N8; ++nt) {
+                  k2[nt][0] = kb[nt >> 1][nt & 1][x2][0];
+                  k2[nt][1] = kb[nt >> 1][nt & 1][x2][1];
+                }
+                score_hl(c, x2, k2);
+              } else {
 #pragma unroll
                 for (int nt = 0; nt < N8; ++nt) {
                   const uint32_t* k2 = kb[nt >> 1][nt & 1][x2];
-                  if (x2 == 0) mma_first<true>(d[nt], ql[x2], k2[0], k2[1]);
-                  else mma_f16(d[nt], ql[x2], k2[0], k2[1]);
+                  if (x2 == 0) mma_first<true>(c[nt], qa[x2], k2[0], k2[1]);
+                  else mma_f16(c[nt], qa[x2], k2[0], k2[1]);
                 }
               }
-#pragma unroll
-              for (int nt = 0; nt < N8; ++nt) {
-                const uint32_t* k2 = kb[nt >> 1][nt & 1][x2];
-                if (x2 == 0) mma_first<true>(c[nt], qa[x2], k2[0], k2[1]);
-                else mma_f16(c[nt], qa[x2], k2[0], k2[1]);
-              }
             }
-          }
-          if constexpr (C::QHL) {
-#pragma unroll
-            for (int nt = 0; nt < N8; ++nt)
-#pragma unroll
-              for (int f = 0; f < 2 * RH; ++f) c[nt][f] += d[nt][f];
           }
 #pragma unroll
           for (int nt = 0; nt < N8; ++nt) {
@@ -672,7 +682,10 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
 #pragma unroll
           for (int nt = 0; nt < N8; ++nt)
 #pragma unroll
-            for (int e = 0; e < RH; ++e) s[nt][e] = fma2(s[nt][e], both(rq[e]), one_r);
+            for (int e = 0; e < RH; ++e) {
+              if constexpr (C::QHL) s[nt][e] = fma2(fma2(s[nt][e], both(rq[e]), both(1.f)), nr, one);
+              else s[nt][e] = fma2(s[nt][e], both(rq[e]), one_r);
+            }
           // NaN (an unseen row, a non-finite key) counts as 0
 #pragma unroll
           for (int nt = 0; nt < N8; ++nt)
