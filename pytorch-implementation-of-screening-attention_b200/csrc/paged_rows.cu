@@ -36,7 +36,8 @@ __device__ __forceinline__ RowBlock row_block(int B, int H, int n, int tokens) {
 // ---------------------------------------------------------------------------
 // Append to int8 pages.  D * sizeof(T) bytes in, D + 4 out per row; bound by issue
 // before HBM, so two elements go through an instruction where one takes pairs,
-// and a token's place in the pages is looked up once for all its heads.
+// and a token's place in the pages is looked up once for all its heads: 4 x 4097
+// tokens of 16 x 64 in bf16 take 29 us (16 us of traffic), 44 without either.
 // ---------------------------------------------------------------------------
 // The bits of the largest magnitude among the row whose 16-byte parts G lanes hold.
 template <typename T, int G>
@@ -122,7 +123,8 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(screen_paged_append_a
 }
 
 // ---------------------------------------------------------------------------
-// Read back: out (B, n, H, D) contiguous, 16 bytes of it a lane.
+// Read back: out (B, n, H, D) contiguous, 16 bytes of it a lane.  Bound by HBM: 4 x
+// 4097 tokens of 16 x 64 in fp32 take 30 us (26 us of traffic).
 // ---------------------------------------------------------------------------
 template <typename E, int N>
 __device__ __forceinline__ void row_n(const E* p, float (&x)[N]) {
@@ -199,7 +201,9 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(screen_paged_read_
 // Commit: row lens[b] + path[b, i] -> lens[b] + i for i < counts[b], one CTA
 // per (layer, K / V, sequence, head).  All source rows are staged in shared
 // memory before the first write, so any path is right, and rows that stay
-// where they are (a chain's) are not touched.
+// where they are (a chain's) are not touched.  Bound by latency: lengths, path, table
+// and rows one after another, 3.6 us for 12 layers of a tree of 16 on bf16 pages, 8.2
+// us for 64 rows on int8 pages (2 us of traffic).
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(128) commit_kernel(screen_commit_args a, int row_bytes) {
   pdl_wait();

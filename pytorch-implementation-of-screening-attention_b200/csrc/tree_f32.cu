@@ -7,7 +7,8 @@ namespace {
 
 // fp32 pages keep the 1e-4 contract of the fp32 path with plain fp32 FMAs: 32
 // keys at a time in shared memory, one (query, key) score per thread and step,
-// then alpha V with the threads over (query group, d).
+// then alpha V with the threads over (query group, d).  Bound by the FMAs and the
+// shared-memory reads that feed them.
 constexpr int kKeys = 32;
 
 template <int D>

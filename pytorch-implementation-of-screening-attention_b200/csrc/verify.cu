@@ -22,6 +22,10 @@
 // parts; a big batch of trees (33 rows each, of which a walk passes two or
 // three) is read row by row as the walk gets there.
 //
+// Bound by the passes of a walk, one after another, each a row through the 64-bit
+// units of a cluster's SMs: 4 chains of 4 with drafting logits over 50257 tokens 24
+// us, 32 trees of 32 34 us.
+//
 // Sums are in 64 bits throughout: with 50K tokens of probability 1e-5 a running
 // sum in 32 bits would often cross u one token away, and an acceptance test next
 // to equality would tip.  The exponentials are good to 2^-31, which moves the

@@ -217,3 +217,46 @@ def test_drafts_are_verified_against_the_rows_they_were_drawn_from(ms, monkeypat
     logits, rows = next((x, r) for x, r in seen if r is not None)
     assert logits.dtype == rows.dtype == torch.float32
     assert torch.equal(torch.cat(drawn, 1), rows)
+
+
+@pytest.mark.parametrize("quantize", [None, "int8"])
+def test_serving_loop_of_trees_equals_greedy_generation(ms, quantize):
+    """Trees step, are verified and committed round after round, three sequences of
+    different progress in one batch, one of them an empty place."""
+    m = lm(ms, torch.float32)
+    B, T, new, n = 3, 19, 30, 8
+    g = torch.Generator(device=DEV).manual_seed(6)
+    ids = torch.randint(0, 97, (B, T), device=DEV, generator=g)
+    want = m.generate(ids, new + n, top_k=1, cache_quantize=quantize)
+    cache = m.make_cache(B, T + new + 2 * n, quantize=quantize, max_draft=n - 1)
+    lens = torch.full((B,), T, dtype=torch.int32, device=DEV)
+    last = m.prefill(ids, cache).argmax(-1)
+    lens[2] = -1                                        # nobody sits there
+    got = [[int(last[b])] for b in range(B)]
+    parents = torch.tensor([[-1, 0, 0, 1, 1, 4, 5, 2]] * B, dtype=torch.int32, device=DEV)
+    parents[1, 5:] = -2                                 # a smaller tree
+    good = [[0, 1, 4, 5, 6], [0, 2, 7]]                 # the true tokens sit on one of these paths
+    counted = 0
+    for turn in range(2 * new):
+        if min(len(got[b]) for b in range(2)) >= new:
+            break
+        tokens = torch.randint(0, 97, (B, n), device=DEV, generator=g)
+        tokens[:, 0] = last
+        for b in range(2):
+            for k, node in enumerate(good[(turn + b) % 2][:1 + turn % 5]):
+                tokens[b, node] = int(want[b, T + len(got[b]) - 1 + k]) if T + len(got[b]) - 1 + k < want.shape[1] else 0
+        logits = m.tree_step(tokens, lens, cache, parents=parents)
+        u = torch.rand(B, n, device=DEV, generator=g)
+        out, path, counts = ms.verify_drafts(logits, tokens[:, 1:], parents[:, 1:] - 1, u, temperature=0.0)
+        kept = torch.cat([torch.zeros_like(path[:, :1]), path + 1], 1)
+        cache.commit(lens, kept, counts + 1)
+        counted += int(counts[:2].sum())
+        for b in range(2):
+            if len(got[b]) < new:
+                a = int(counts[b])
+                got[b] += out[b, :a + 1].tolist()
+                last[b] = out[b, a]
+                lens[b] += a + 1
+    for b in range(2):
+        assert got[b][:new] == want[b, T:T + new].tolist()
+    assert counted > new // 2                           # drafts were accepted
