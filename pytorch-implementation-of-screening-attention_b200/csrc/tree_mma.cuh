@@ -72,10 +72,15 @@ struct Cfg {
   // them; a lone warp does it on the way into the fragments.
   static constexpr bool CONV = I8 && MG_ > 1;
   static constexpr bool LDM = !I8 || CONV;       // 16-bit tiles read by ldmatrix
-  // fp32 activations: q and alpha as hi + lo halves, fp32 sums between products.
-  // bf16 pages: alpha as hi + lo (one half would round as much as the output).
+  // alpha enters the product as hi + lo halves: 2^-22 of it over int8 pages (fp16),
+  // 2^-18 over bf16 pages, next to V rows rounded at 2^-9 there and scores whose
+  // 32-bit sums are good to about as much.  One half alone would be off by 2^-12 /
+  // 2^-9, which shows wherever values cancel.
+  // fp32 activations: q as hi + lo too, fp32 sums between products.
   static constexpr bool QHL = I8 && sizeof(TA_) == 4;
-  static constexpr bool PHL = QHL || !I8;
+  // up to 8 queries leave the lower rows of a tile free: the lo halves go there, in
+  // the same product
+  static constexpr bool SPARE = I8 && !QHL && RH_ == 1;
   static constexpr int RB = D_ * (int)sizeof(E_);     // row bytes
   static constexpr int CH = RB / 16;                  // 16-byte chunks per row
   static constexpr int CH16 = D_ / 8;                 // of a 16-bit row
@@ -101,7 +106,7 @@ struct Cfg {
   // CTAs per SM the registers are cut to: what a thread holds of O and q decides
   static constexpr int HELD = D_ / 2 + D_ / 4 * (QHL ? 2 : 1);
   // (a group of four warps on int8 pages waits at its barriers and gains by a fourth
-  // CTA: 64 nodes over 32K keys 142 us, 148 with three)
+  // CTA: 64 nodes over 32K keys 157 us, 160 with three)
   static constexpr int MINB =
       HELD <= 32 ? 4 : HELD <= 64 ? (CONV && MG_ == 4 && !QHL ? 4 : 3) : 2;
 };
@@ -283,8 +288,8 @@ __device__ __forceinline__ void widen16(uint4 u, uint4& lo, uint4& hi) {
 //
 // A group of one warp (up to 16 nodes) is bound by its issue and its waits before
 // HBM: one query per sequence over 100K int8 keys of 64 heads 122 us, 4.5 TB/s.  64
-// nodes over 32K int8 keys 135 us, 159 TFLOP/s, half of the issue slots and 30 % of
-// mma.sync used (430 instructions a warp per 32 keys x 16 nodes).  16 nodes over
+// nodes over 32K int8 keys 157 us, 137 TFLOP/s (135 us with alpha as one fp16 number,
+// whose rounding showed where values cancel).  16 nodes over
 // windows of 4K on bf16 pages 24 us, 8.2 us for one token over 256 int8 keys: latency.
 template <class C>
 __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams p,
@@ -790,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
 #pragma unroll
         for (int kg = 0; kg < C::NK; ++kg) {
           if (!live[kg]) continue;
-          // a fragment's registers: row half e of 8-key tile nt
+          // a fragment's registers: row half e of 8-key tile nt; SPARE: row half 1 is lo
           uint32_t pa[4] = {0u, 0u, 0u, 0u}, pl[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt)
@@ -799,11 +804,10 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
               const int f = 2 * nt + e;
               const float2 v = al[2 * kg + nt][e];
               pa[f] = C::I8 ? pack_f16(v.x, v.y) : pack_bf16(v.x, v.y);
-              if constexpr (C::PHL) {
-                const float2 u = C::I8 ? __half22float2(*reinterpret_cast<__half2*>(&pa[f]))
-                                       : unpack_bf16(pa[f]);
-                pl[f] = C::I8 ? pack_f16(v.x - u.x, v.y - u.y) : pack_bf16(v.x - u.x, v.y - u.y);
-              }
+              const float2 u = C::I8 ? __half22float2(*reinterpret_cast<__half2*>(&pa[f]))
+                                     : unpack_bf16(pa[f]);
+              (C::SPARE ? pa[f | 1] : pl[f]) =
+                  C::I8 ? pack_f16(v.x - u.x, v.y - u.y) : pack_bf16(v.x - u.x, v.y - u.y);
             }
           uint32_t vb[C::NT][2];
           load_v<C>(vt, kg * 16, lane, vb);
@@ -829,6 +833,10 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
               for (int f = 0; f < 2 * RH; ++f) o[j][f] += d[f];
             }
           } else if constexpr (C::I8) {
+            if constexpr (!C::SPARE) {
+#pragma unroll
+              for (int j = 0; j < C::NT; ++j) mma_f16(o[j], pl, vb[j][0], vb[j][1]);
+            }
 #pragma unroll
             for (int j = 0; j < C::NT; ++j) mma_f16(o[j], pa, vb[j][0], vb[j][1]);
           } else {
@@ -861,7 +869,7 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
     for (int j = 0; j < C::NT; ++j)
 #pragma unroll
       for (int f = 0; f < 2; ++f)
-        dst[o_col<C>(j, 2 * t + f)] = o[j][2 * e + f] * back;
+        dst[o_col<C>(j, 2 * t + f)] = (C::SPARE ? o[j][f] + o[j][2 + f] : o[j][2 * e + f]) * back;
   }
   __syncthreads();
   if (!whole) {

@@ -367,3 +367,50 @@ def test_runs_shorter_than_a_tree(ms, dtype, q8, n, T):
     lens = torch.tensor([T, max(0, T - 9)], dtype=torch.int32)
     r, w = torch.tensor([1.1, 1.4]), torch.tensor([400.0, 20.0])
     check(ms, c, lens, tree_parents(2, n, "random", c["g"]), r, w, dtype, q8, num_ctas=592)
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, True), (torch.bfloat16, False), (torch.float32, True)])
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("n", [0, 1, 5, 12, 20, 40])
+def test_values_that_cancel(ms, n, D, dtype, q8):
+    """Pairs of nearly equal keys with opposite values: what is left of the sum is
+    far below its terms, so that the output's rounding hides nothing of alpha's.
+    alpha is held to 2^-21 (two fp16 halves, 2^-11 each, the rest sums in 32 bits),
+    to 2^-17 over bf16 pages (two bf16 halves, 2^-9 each).  n = 0: one query."""
+    B, H, T, ps = 2, 8, 16, 16
+    g = torch.Generator().manual_seed(100 * n + D)
+    k = torch.randn(B, T // 2, H, D, generator=g).repeat_interleave(2, 1)
+    k = k + 0.003 * torch.randn(B, T, H, D, generator=g)
+    v = torch.randn(B, T // 2, H, D, generator=g).repeat_interleave(2, 1)
+    v[:, 1::2] *= -1
+    mean = 2.0 * torch.randn(H, D, generator=g)
+    k = (k + mean).to(dtype)
+    q = (mean + torch.randn(B, max(n, 1), H, D, generator=g)).to(dtype)
+    blocks = (T + n) // ps + 1
+    table = torch.randperm(B * blocks, generator=g).view(B, blocks).to(torch.int32).to(DEV)
+    kp = torch.zeros(B * blocks, H, ps, D, dtype=torch.int8 if q8 else dtype, device=DEV)
+    vp = torch.zeros_like(kp)
+    ks, vs = [torch.zeros(B * blocks, H, ps, device=DEV) if q8 else None for _ in range(2)]
+    ms.paged_append(k.to(DEV), v.to(dtype).to(DEV), torch.zeros(B, dtype=torch.int32, device=DEV), kp, vp, table, ks, vs)
+    prefix = [None if x is None else x.cpu().clone() for x in (kp, vp, ks, vs, table)]
+    r, w = torch.full((H,), 1.05), torch.full((H,), 4000.0)
+    lens = torch.full((B,), T, dtype=torch.int32, device=DEV)
+    if n:
+        # a node's own key is the opposite of what the queries lean on: trimmed
+        own = (-mean).expand(B, n, H, D).to(dtype)
+        y = ms.paged_tree_decode(q.to(DEV), own.to(DEV), own.to(DEV), lens, None, r.to(DEV), w.to(DEV), kp, vp, table, ks, vs)
+    else:
+        y = ms.paged_decode(q[:, 0].to(DEV), lens, r.to(DEV), w.to(DEV), kp, vp, table, ks, vs)[:, None]
+    al = 2.0**-21 if q8 else 2.0**-17
+    out = 2.0**-8 if dtype == torch.bfloat16 else 2.0**-22
+    for b in range(B):
+        pk, pv = (po.cache_values(prefix[i], prefix[i + 2], prefix[4], b, list(range(T))) for i in (0, 1))
+        for i in range(max(n, 1)):
+            back = torch.arange(T - 1, -1, -1) + (i + 1 if n else 0)
+            for h in range(H):
+                want, s = po.query(q[b, i, h], pk[:, h], pv[:, h], back, float(r[h]), float(w[h]))
+                lim = out * want.norm() + al * s[0] + 2.0**-18 * 1.05 * s[1] + 2.0**-21 * s[2] + 1e-9
+                err = (y[b, i, h].double().cpu() - want).norm()
+                assert err <= lim, (b, i, h, float(err), float(lim))
+                if D == 64:
+                    assert s[0] > 20 * want.norm()          # the terms do cancel
