@@ -72,15 +72,14 @@ struct Cfg {
   // them; a lone warp does it on the way into the fragments.
   static constexpr bool CONV = I8 && MG_ > 1;
   static constexpr bool LDM = !I8 || CONV;       // 16-bit tiles read by ldmatrix
-  // alpha enters the product as hi + lo halves: 2^-22 of it over int8 pages (fp16),
-  // 2^-18 over bf16 pages, next to V rows rounded at 2^-9 there and scores whose
-  // 32-bit sums are good to about as much.  One half alone would be off by 2^-12 /
-  // 2^-9, which shows wherever values cancel.
+  // alpha enters the product whole: as two fp16 numbers over int8 pages (2^-22 of
+  // it), as three bf16 numbers over bf16 pages (2^-24).  One fp16 or two bf16 numbers
+  // (2^-11, 2^-16) show wherever values cancel.
   // fp32 activations: q as hi + lo too, fp32 sums between products.
   static constexpr bool QHL = I8 && sizeof(TA_) == 4;
-  // up to 8 queries leave the lower rows of a tile free: the lo halves go there, in
-  // the same product
-  static constexpr bool SPARE = I8 && !QHL && RH_ == 1;
+  // up to 8 queries leave the lower rows of a tile free: alpha's second numbers go
+  // there, in the same product as the first
+  static constexpr bool SPARE = !QHL && RH_ == 1;
   static constexpr int RB = D_ * (int)sizeof(E_);     // row bytes
   static constexpr int CH = RB / 16;                  // 16-byte chunks per row
   static constexpr int CH16 = D_ / 8;                 // of a 16-bit row
@@ -795,19 +794,27 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
 #pragma unroll
         for (int kg = 0; kg < C::NK; ++kg) {
           if (!live[kg]) continue;
-          // a fragment's registers: row half e of 8-key tile nt; SPARE: row half 1 is lo
-          uint32_t pa[4] = {0u, 0u, 0u, 0u}, pl[4] = {0u, 0u, 0u, 0u};
+          // a fragment's registers: row half e of 8-key tile nt; SPARE: pl's in row half 1
+          uint32_t pa[4] = {0u, 0u, 0u, 0u}, pl[4] = {0u, 0u, 0u, 0u}, pm[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
             for (int e = 0; e < RH; ++e) {
               const int f = 2 * nt + e;
               const float2 v = al[2 * kg + nt][e];
-              pa[f] = C::I8 ? pack_f16(v.x, v.y) : pack_bf16(v.x, v.y);
-              const float2 u = C::I8 ? __half22float2(*reinterpret_cast<__half2*>(&pa[f]))
-                                     : unpack_bf16(pa[f]);
-              (C::SPARE ? pa[f | 1] : pl[f]) =
-                  C::I8 ? pack_f16(v.x - u.x, v.y - u.y) : pack_bf16(v.x - u.x, v.y - u.y);
+              uint32_t& second = C::SPARE ? pa[f | 1] : pl[f];
+              if constexpr (C::I8) {
+                pa[f] = pack_f16(v.x, v.y);
+                const float2 u = __half22float2(*reinterpret_cast<__half2*>(&pa[f]));
+                second = pack_f16(v.x - u.x, v.y - u.y);
+              } else {
+                pa[f] = pack_bf16(v.x, v.y);
+                float2 u = unpack_bf16(pa[f]);
+                const float2 d = make_float2(v.x - u.x, v.y - u.y);
+                second = pack_bf16(d.x, d.y);
+                u = unpack_bf16(second);
+                pm[f] = pack_bf16(d.x - u.x, d.y - u.y);
+              }
             }
           uint32_t vb[C::NT][2];
           load_v<C>(vt, kg * 16, lane, vb);
@@ -841,7 +848,11 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
             for (int j = 0; j < C::NT; ++j) mma_f16(o[j], pa, vb[j][0], vb[j][1]);
           } else {
 #pragma unroll
-            for (int j = 0; j < C::NT; ++j) mma_b16(o[j], pl, vb[j][0], vb[j][1]);
+            for (int j = 0; j < C::NT; ++j) mma_b16(o[j], pm, vb[j][0], vb[j][1]);
+            if constexpr (!C::SPARE) {
+#pragma unroll
+              for (int j = 0; j < C::NT; ++j) mma_b16(o[j], pl, vb[j][0], vb[j][1]);
+            }
 #pragma unroll
             for (int j = 0; j < C::NT; ++j) mma_b16(o[j], pa, vb[j][0], vb[j][1]);
           }

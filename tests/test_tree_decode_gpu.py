@@ -414,3 +414,45 @@ def test_values_that_cancel(ms, n, D, dtype, q8):
                 assert err <= lim, (b, i, h, float(err), float(lim))
                 if D == 64:
                     assert s[0] > 20 * want.norm()          # the terms do cancel
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, True), (torch.bfloat16, False), (torch.float32, True),
+                                      (torch.float32, False)])
+@pytest.mark.parametrize("D", [16, 64])
+@pytest.mark.parametrize("n", [1, 5, 12, 20, 40])
+def test_alpha_is_held_whole(ms, n, D, dtype, q8):
+    """Two equal keys, one place apart, with opposite values: their scores are the
+    same number, so what is left is the difference of the masks (2^-17 of either) and
+    the roundings of alpha after the score.  Those are at most, in half steps 2^-24:
+    the cosine and sine (2 each, weight 1/2), their products with the V row's scale and
+    the node's factors (3), two sums, the product with t^2 (1), and 4 for two fp16
+    numbers (three bf16 numbers: 1): 12 an alpha, held to 16."""
+    B, H, T, ps = 2, 16, 2, 16
+    g = torch.Generator().manual_seed(10 * n + D)
+    lead = torch.zeros(H, D)
+    lead[:, 0] = 1.0
+    k = lead + 0.6 * torch.rand(B, 1, H, D, generator=g) / math.sqrt(D)
+    k = k.expand(B, T, H, D).contiguous()
+    v = torch.randn(B, 1, H, D, generator=g)
+    v = torch.cat([v, -v], 1)
+    q = lead.expand(B, n, H, D)
+    own = -q
+    blocks = (T + n) // ps + 1
+    table = torch.randperm(B * blocks, generator=g).view(B, blocks).to(torch.int32).to(DEV)
+    kp = torch.zeros(B * blocks, H, ps, D, dtype=torch.int8 if q8 else dtype, device=DEV)
+    vp = torch.zeros_like(kp)
+    ks, vs = [torch.zeros(B * blocks, H, ps, device=DEV) if q8 else None for _ in range(2)]
+    k, v, q, own = (x.to(dtype).to(DEV) for x in (k, v, q, own))
+    ms.paged_append(k, v, torch.zeros(B, dtype=torch.int32, device=DEV), kp, vp, table, ks, vs)
+    prefix = [None if x is None else x.cpu().clone() for x in (kp, vp, ks, vs, table)]
+    r, w = torch.full((H,), 1.0625), torch.full((H,), 4000.0)
+    lens = torch.full((B,), T, dtype=torch.int32, device=DEV)
+    y = ms.paged_tree_decode(q, own, own, lens, None, r.to(DEV), w.to(DEV), kp, vp, table, ks, vs)
+    out = 2.0**-8 if dtype == torch.bfloat16 else 2.0**-22
+    for b in range(B):
+        pk, pv = (po.cache_values(prefix[i], prefix[i + 2], prefix[4], b, list(range(T))) for i in (0, 1))
+        for i in range(n):
+            for h in range(H):
+                want, s = po.query(q[b, i, h], pk[:, h], pv[:, h], torch.tensor([i + 2, i + 1]), float(r[h]), float(w[h]))
+                err = (y[b, i, h].double().cpu() - want).norm()
+                assert s[0] > 1.0 and err <= out * want.norm() + 2.0**-20 * s[0], (b, i, h, float(err), s[0])
