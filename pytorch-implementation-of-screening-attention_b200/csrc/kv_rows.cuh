@@ -144,9 +144,11 @@ __device__ __forceinline__ void int8_pack(float (&x)[E], const Int8Scale& s, uin
 }
 // The stored scale of a row, ss = |m|^2.
 __device__ __forceinline__ float int8_stored_scale(uint32_t top, int ss, float eps) {
-  // 1 / |m| by one Newton step from the approximate reciprocal root
+  // 1 / |m| by one Newton step from the approximate reciprocal root, the product
+  // n2 y with its rounding error, so that only the last sum rounds
   const float amax = __uint_as_float(top), n2 = (float)ss, y = rsqrtf(n2);
-  float scale = fmaf(0.5f * y, fmaf(-n2 * y, y, 1.0f), y);
+  const float p = n2 * y, low = fmaf(n2, y, -p);
+  float scale = fmaf(0.5f * y, fmaf(-low, y, fmaf(-p, y, 1.0f)), y);
   // |m| >= 127: only a row below eps can meet the other bound, 1 / max(a, b) as
   // min(1 / a, 1 / b)
   if (!(amax >= eps)) scale = top ? fminf(scale, amax / (127.0f * eps)) : 0.f;

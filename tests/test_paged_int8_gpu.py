@@ -192,3 +192,18 @@ def test_every_bf16_quotient(ms):
     want = (q + ((2 * rest > den) | ((2 * rest == den) & (q % 2 == 1))).long()) * rows.sign().long()
     for pages in (kp, vp):
         assert torch.equal(pages[table[0].long()].cpu().view(1024, 128).long(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [16, 64, 128])
+def test_scales_are_rounded_once(ms, dtype, D):
+    """|m|^2 is a whole number below 2^21, exact in 32 bits; 1 / |m| is off by one
+    rounding (2^-24) and 2^-44, the square of the approximate root's error."""
+    n, H = 500, 8
+    x = torch.randn(1, n, H, D, generator=torch.Generator().manual_seed(D)).to(dtype)
+    kp, vp, table, ks, vs = empty_cache(1, H, D, 64, n // 64 + 1)
+    ms.paged_append(x.to(DEV), x.flip(1).to(DEV), torch.zeros(1, dtype=torch.int32, device=DEV), kp, vp, table, ks, vs)
+    for scales, rows in ((ks, x), (vs, x.flip(1))):
+        _, want = po.int8_rows(rows[0])                                          # (n, H)
+        got = scales[table[0].long()].transpose(1, 2).reshape(-1, H)[:n].double().cpu()
+        assert ((got - want).abs() <= (1 + 2.0**-16) * 2.0**-24 * want).all()
