@@ -64,8 +64,9 @@ __device__ __forceinline__ void load8f(const T* p, float (&x)[8]) {
 // with the approximate reciprocal and one remainder step leave the quotient right
 // to 2^-24 (its nearest float, but for 2^-44 of it): a half comes out exactly, and
 // no other quotient of 8-bit significands lies within 2^-17 of one; for fp32 a quotient so near a half
-// that 32 bits cannot tell (127 * 2^-23 at most; one in 16,000) is decided by an
-// exact comparison in 64 bits.  A row with an infinity or NaN becomes m = 0, scale
+// that 32 bits cannot tell is decided by an exact comparison in 64 bits: three roundings
+// of 2^-24 of up to 127 move it by 2.3e-5, and what lies within 2^-15 = 3.1e-5 of a
+// half (one in 16,000) is compared.  A row with an infinity or NaN becomes m = 0, scale
 // NaN.
 struct Int8Scale {
   float up, am, inv;     // x is scaled by up (0: a row of zeros); am = max|up x|

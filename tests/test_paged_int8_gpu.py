@@ -207,3 +207,25 @@ def test_scales_are_rounded_once(ms, dtype, D):
         _, want = po.int8_rows(rows[0])                                          # (n, H)
         got = scales[table[0].long()].transpose(1, 2).reshape(-1, H)[:n].double().cpu()
         assert ((got - want).abs() <= (1 + 2.0**-16) * 2.0**-24 * want).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("H", [40, 150])
+def test_more_heads_than_a_block_moves_at_once(ms, dtype, H):
+    """A token's heads go through a block in several turns."""
+    B, n, D, ps = 2, 3, 128, 16
+    g = torch.Generator().manual_seed(H)
+    k, v = (torch.randn(B, n, H, D, generator=g).to(dtype) for _ in range(2))
+    pos = torch.tensor([14, 3], dtype=torch.int32)
+    kp, vp, table, ks, vs = empty_cache(B, H, D, ps, 2)
+    ms.paged_append(k.to(DEV), v.to(DEV), pos.to(DEV), kp, vp, table, ks, vs)
+    got = ms.paged_read(pos.to(DEV), n, kp, vp, table, ks, vs)
+    for raw, pages, scales, val in ((k, kp, ks, got[0]), (v, vp, vs, got[1])):
+        m, sc = po.int8_rows(raw)
+        for b in range(B):
+            p = torch.arange(n) + int(pos[b])
+            page = table[b].cpu().long()[p // ps]
+            assert torch.equal(pages[page.to(DEV), :, (p % ps).to(DEV)].cpu(), m[b])
+        want = m.double() * sc[..., None]
+        assert ((val.double().cpu() - want).abs() <= 4 * 2.0**-24 * want.abs()).all()
+    assert int((kp != 7).any(-1).sum()) <= B * n * H
