@@ -12,6 +12,7 @@ prefix for every token (multiscreen/model.py:131-133).
 """
 from __future__ import annotations
 
+import math
 import struct
 
 import torch
@@ -238,7 +239,7 @@ def _tree_ctas(bh: int, keys: int) -> int:
 
 def _keys_seen(max_window, block_table, page_size):
     table = block_table.shape[1] * page_size
-    return table if not max_window or max_window <= 0 else min(int(-(-max_window // 1)), table)
+    return math.ceil(max_window) if max_window and 0 < max_window < table else table
 
 
 def _tree(name, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_scales, v_scales,

@@ -456,3 +456,16 @@ def test_alpha_is_held_whole(ms, n, D, dtype, q8):
                 want, s = po.query(q[b, i, h], pk[:, h], pv[:, h], torch.tensor([i + 2, i + 1]), float(r[h]), float(w[h]))
                 err = (y[b, i, h].double().cpu() - want).norm()
                 assert s[0] > 1.0 and err <= out * want.norm() + 2.0**-20 * s[0], (b, i, h, float(err), s[0])
+
+
+@pytest.mark.parametrize("hint", [math.inf, math.nan, -1.0])
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)])
+def test_hints_of_any_window(ms, dtype, q8, hint):
+    """max_window only sets how the work is shared out: inf (a head that sees all) is
+    one."""
+    c = make(ms, 2, 2, 64, 16, 70, 4, dtype, q8, 6)
+    lens = torch.tensor([70, 50], dtype=torch.int32)
+    r, w = torch.tensor([1.1, 1.4]), torch.tensor([1e9, 20.0])
+    check(ms, c, lens, None, r, w, dtype, q8, max_window=hint)
+    args = (c["q"][:, 0].to(DEV), (lens + 1).to(DEV), r.to(DEV), w.to(DEV), c["kp"], c["vp"], c["table"], c["ks"], c["vs"])
+    assert torch.equal(ms.paged_decode(*args, max_window=hint), ms.paged_decode(*args))
