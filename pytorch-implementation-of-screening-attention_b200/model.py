@@ -388,8 +388,8 @@ class MultiscreenLM(nn.Module):
         def draw(n):
             return torch.rand(B, n, device=dev, generator=generator)
 
-        last, _, _ = verify_drafts(logits.unsqueeze(1), input_ids.new_empty((B, 0)), None, draw(1),
-                                   temperature=temperature)
+        none = torch.empty((B, 0), dtype=torch.long, device=dev)      # the prompt may be int32
+        last, _, _ = verify_drafts(logits.unsqueeze(1), none, None, draw(1), temperature=temperature)
         lens = torch.full((B,), T0, dtype=torch.int32, device=dev)
         made = torch.ones(B, dtype=torch.long, device=dev)
         new = torch.zeros(B, max_new_tokens + num_draft + 1, dtype=torch.long, device=dev)

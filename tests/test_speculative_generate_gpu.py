@@ -260,3 +260,13 @@ def test_serving_loop_of_trees_equals_greedy_generation(ms, quantize):
     for b in range(2):
         assert got[b][:new] == want[b, T:T + new].tolist()
     assert counted > new // 2                           # drafts were accepted
+
+
+@pytest.mark.parametrize("graph", [True, False])
+def test_int32_prompts(ms, graph):
+    """A prompt may be int32, as for generate()."""
+    m, d = lm(ms, torch.float32), lm(ms, torch.float32, layers=1)
+    ids = torch.randint(0, 97, (2, 17), device=DEV)
+    want = m.generate(ids.int(), 9, top_k=1)
+    got = m.generate_speculative(ids.int(), d, 9, num_draft=3, temperature=0.0, cuda_graph=graph)
+    assert got.dtype == want.dtype and torch.equal(got, want)
