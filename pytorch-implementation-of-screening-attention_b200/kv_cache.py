@@ -61,20 +61,7 @@ class PagedKVCache:
                  + (lb % self.pages_per_seq).unsqueeze(0))
         self.block_table = table.to(device)
         self._workspace = None
-        # split each (b, h) window into runs of whole pages: at least one
-        # wave of CTAs (148 SMs x 3 resident decode CTAs), and about
-        # sqrt(pages) splits for long windows -- measured on B200 at 32K and
-        # 100K keys per window, fewer splits leave a wave tail, more pay the
-        # per-CTA pipeline fill; the split partials are summed
-        # short windows (<= 512 keys: the w <= 256 of a model at init) take
-        # one split per (b, h), which applies TanhNorm itself: a finishing
-        # launch costs more than the few pages it would spread
-        pages = math.ceil(self.keep / page_size)
-        fill = math.ceil(148 * 3 / max(1, batch * num_heads))
-        if self.keep <= 512:
-            self.num_splits = 1
-        else:
-            self.num_splits = max(1, min(256, pages, max(fill, round(1.1 * math.sqrt(pages)))))
+        self.num_splits = paged.decode_splits(batch * num_heads, self.keep, page_size)
 
     def nbytes(self) -> int:
         every = self.k_pages + self.v_pages + [t for t in self.k_scales + self.v_scales

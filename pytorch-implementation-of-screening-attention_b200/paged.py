@@ -242,6 +242,21 @@ def _keys_seen(max_window, block_table, page_size):
     return math.ceil(max_window) if max_window and 0 < max_window < table else table
 
 
+def decode_splits(pairs: int, keys: int, page_size: int) -> int:
+    """Splits per (sequence, head) of a decode over fp32 / bf16 pages: runs of whole
+    pages, at least one wave of CTAs (148 SMs x 3 resident decode CTAs), and about
+    sqrt(pages) for long windows -- measured at 32K and 100K keys per window, fewer
+    leave a wave tail, more pay the per-CTA pipeline fill (4 x 16 heads of 64 over 100K
+    bf16 keys, windows from a quarter on: 185 us with 43 splits, 262 with 10).  Windows of up to 512 keys
+    (the w <= 256 of a model at init) take one, which applies TanhNorm itself: a
+    finishing launch costs more than the few pages it would spread."""
+    if keys <= 512:
+        return 1
+    pages = math.ceil(keys / page_size)
+    fill = math.ceil(148 * 3 / max(1, pairs))
+    return max(1, min(256, pages, max(fill, round(1.1 * math.sqrt(pages)))))
+
+
 def _tree(name, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_scales, v_scales,
           max_window, num_ctas, eps):
     """q, k, v (B, n, H, D); or q (B, H, D), one query per sequence."""
@@ -320,9 +335,9 @@ def paged_decode(q, seq_lens, r, w, k_pages, v_pages, block_table, k_scales=None
         r, w = _head_params(r, w, H, index)
         keys = _keys_seen(max_window, block_table, shape[2])
         if num_ctas is None:
-            num_ctas = _tree_ctas(B * H, keys)
-        # splits of every (sequence, head), at least a page each
-        num_splits = max(1, min(-(-num_ctas // max(1, B * H)), -(-keys // shape[2])))
+            num_splits = decode_splits(B * H, keys, shape[2])
+        else:                    # of every (sequence, head), at least a page each
+            num_splits = max(1, min(-(-num_ctas // max(1, B * H)), -(-keys // shape[2])))
         with torch.cuda.device(index):
             return _lib.screen_decode(q.detach(), seq_lens, r, w, k_pages, v_pages, block_table,
                                       eps, num_splits)[0]

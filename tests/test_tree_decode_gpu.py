@@ -469,3 +469,21 @@ def test_hints_of_any_window(ms, dtype, q8, hint):
     check(ms, c, lens, None, r, w, dtype, q8, max_window=hint)
     args = (c["q"][:, 0].to(DEV), (lens + 1).to(DEV), r.to(DEV), w.to(DEV), c["kp"], c["vp"], c["table"], c["ks"], c["vs"])
     assert torch.equal(ms.paged_decode(*args, max_window=hint), ms.paged_decode(*args))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [400, 12000])
+def test_decode_is_the_cache_s_decode(ms, dtype, T):
+    """paged_decode over a PagedKVCache's pages shares out its work as the cache's own
+    decode does: the same bits."""
+    B, H, D = 4, 16, 64
+    g = torch.Generator().manual_seed(T)
+    cache = ms.PagedKVCache(1, B, H, D, T + 10, float(T), dtype, DEV)
+    k, v = ((torch.randn(B, T, H, D, generator=g) + 0.5).to(dtype).to(DEV) for _ in range(2))
+    cache.append(0, k, v, torch.zeros(B, dtype=torch.int32, device=DEV))
+    q = (k[:, -1].cpu() + 0.5 * torch.randn(B, H, D, generator=g)).to(dtype).to(DEV)
+    lens = torch.tensor([T, T - 37, T // 2, 1], dtype=torch.int32, device=DEV)
+    r, w = torch.full((H,), 1.1, device=DEV), torch.linspace(float(T), 50.0, H).to(DEV)
+    want, _ = cache.decode(0, q, lens, r, w)
+    got = ms.paged_decode(q, lens, r, w, cache.k_pages[0], cache.v_pages[0], cache.block_table, max_window=float(T))
+    assert torch.equal(got, want)
