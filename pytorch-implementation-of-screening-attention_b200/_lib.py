@@ -548,7 +548,8 @@ def screen_decode(q, seq_lens, r, w, k_pages, v_pages, block_table, eps=1e-8, nu
     _require_cuda(q, seq_lens, r, w, k_pages, v_pages, block_table)
     lib = load()
     if q.stride(-1) != 1 or q.stride(-2) != q.shape[-1] or q.stride(0) % 4 or q.data_ptr() % 16:
-        q = q.contiguous()
+        # a copy even where torch counts q as contiguous: it may start anywhere
+        q = q.clone(memory_format=torch.contiguous_format)
     B, H, D = q.shape
     dev = q.device
     y = torch.empty((B, H, D), dtype=q.dtype, device=dev)
@@ -578,7 +579,8 @@ def screen_decode_append(k, v, positions, q, seq_lens, r, w, k_pages, v_pages, b
     if k_pages.dtype != k.dtype or q.dtype != k.dtype:
         raise TypeError("cache dtype must match q / k / v")
     if q.stride(-1) != 1 or q.stride(-2) != q.shape[-1] or q.stride(0) % 4 or q.data_ptr() % 16:
-        q = q.contiguous()
+        # a copy even where torch counts q as contiguous: it may start anywhere
+        q = q.clone(memory_format=torch.contiguous_format)
     B, H, D = q.shape
     dev = q.device
     cache = kv_desc(k_pages, v_pages, block_table)

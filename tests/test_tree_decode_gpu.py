@@ -487,3 +487,18 @@ def test_decode_is_the_cache_s_decode(ms, dtype, T):
     want, _ = cache.decode(0, q, lens, r, w)
     got = ms.paged_decode(q, lens, r, w, cache.k_pages[0], cache.v_pages[0], cache.block_table, max_window=float(T))
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_decode_queries_that_start_anywhere(ms, dtype):
+    """A contiguous q that does not start on 16 bytes, and a batch of one with any
+    batch stride, are read as any other over fp32 / bf16 pages too."""
+    c = make(ms, 1, 3, 64, 16, 60, 1, dtype, False, 3)
+    r, w = torch.full((3,), 1.2, device=DEV), torch.full((3,), 40.0, device=DEV)
+    tail = (torch.full((1,), 60, dtype=torch.int32, device=DEV), r, w, c["kp"], c["vp"], c["table"])
+    q = c["q"][:, 0].to(DEV)
+    flat = torch.empty(q.numel() + 1, dtype=dtype, device=DEV)
+    flat[1:] = q.flatten()
+    want = ms.paged_decode(q, *tail)
+    assert torch.equal(ms.paged_decode(flat[1:].view(1, 3, 64), *tail), want)
+    assert torch.equal(ms.paged_decode(q.as_strided((1, 3, 64), (7, 64, 1)), *tail), want)
