@@ -108,6 +108,13 @@ struct Cfg {
   // CTA: 64 nodes over 32K keys 157 us, 160 with three)
   static constexpr int MINB =
       HELD <= 32 ? 4 : HELD <= 64 ? (CONV && MG_ == 4 && !QHL ? 4 : 3) : 2;
+  // CTAs resident on an SM: its registers and its 228 KB of shared memory, of which a
+  // CTA takes 1 KB more than it asks for (int8 rows of 128 with 17 to 32 nodes: one;
+  // 32 nodes, 4 x 8 heads, 8K keys 47 us, 56 with runs cut for two; 24 nodes, 4 x 16
+  // heads, 32K keys, where two waves even out the heads, 290 and 275)
+  static constexpr int CTA_B = SMEM + (int)sizeof(Nodes) + 64 + 1024;
+  static constexpr int PER_SM = MINB * CTA_B <= 228 * 1024 ? MINB : 228 * 1024 / CTA_B;
+  static_assert(PER_SM >= 1 && PER_SM * CTA_B <= 228 * 1024, "a grid of PER_SM CTAs an SM is resident at once");
 };
 
 // Byte offset of 16-byte chunk c of row r in a tile: the XOR makes the fragment
@@ -917,7 +924,7 @@ template <class C>
 void launch_tree(const TreeParams& p, float* ws, cudaStream_t s) {
   if (ensure_smem_optin((const void*)tree_mma_kernel<C>, C::SMEM) != cudaSuccess) return;
   prefer_shared((const void*)tree_mma_kernel<C>);
-  launch_pdl(tree_mma_kernel<C>, tree_grid(p, C::MINB), dim3(kThreads), (size_t)C::SMEM, s, p, ws);
+  launch_pdl(tree_mma_kernel<C>, tree_grid(p, C::PER_SM), dim3(kThreads), (size_t)C::SMEM, s, p, ws);
 }
 // A warp for every 16 queries; up to 8 queries the lower half of a tile is not
 // computed on.
