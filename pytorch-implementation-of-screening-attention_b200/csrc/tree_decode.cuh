@@ -354,6 +354,13 @@ inline void prefer_shared(const void* fn) {
   cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
 }
 
+// CTAs that an SM's 228 KB of shared memory hold, `most` of them at most: a CTA takes
+// its own, the static arrays (under 1.5 KB) and 1 KB more.
+constexpr int fit_shared(size_t smem, int most) {
+  const size_t cta = smem + 1536 + 1024, n = 228 * 1024 / cta;
+  return n < (size_t)most ? (int)n : most;
+}
+
 // One CTA per segment, or at most as many as are resident at once (a CTA per segment
 // at least).
 constexpr int kSMs = 148;

@@ -172,7 +172,9 @@ void launch_f32(const TreeParams& p, float* part, cudaStream_t s) {
   constexpr int kMost = (kMaxN * D + 2 * kKeys * (D + 4) + kMaxN * 33) * 4;
   if (ensure_smem_optin((const void*)tree_f32_kernel<D>, kMost) != cudaSuccess) return;
   prefer_shared((const void*)tree_f32_kernel<D>);
-  launch_pdl(tree_f32_kernel<D>, tree_grid(p, 3), dim3(kThreads), smem, s, p, part);
+  // three CTAs an SM where they fit (64 nodes of 128: two)
+  static_assert(sizeof(Nodes) + kKeys * 12 + 64 <= 1536, "the static arrays are counted");
+  launch_pdl(tree_f32_kernel<D>, tree_grid(p, fit_shared(smem, 3)), dim3(kThreads), smem, s, p, part);
 }
 template <typename TA, int D>
 void launch_finish(const TreeParams& p, const float* part, cudaStream_t s) {

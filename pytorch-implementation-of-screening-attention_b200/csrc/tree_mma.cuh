@@ -108,13 +108,11 @@ struct Cfg {
   // CTA: 64 nodes over 32K keys 157 us, 160 with three)
   static constexpr int MINB =
       HELD <= 32 ? 4 : HELD <= 64 ? (CONV && MG_ == 4 && !QHL ? 4 : 3) : 2;
-  // CTAs resident on an SM: its registers and its 228 KB of shared memory, of which a
-  // CTA takes 1 KB more than it asks for (int8 rows of 128 with 17 to 32 nodes: one;
-  // 32 nodes, 4 x 8 heads, 8K keys 47 us, 56 with runs cut for two; 24 nodes, 4 x 16
-  // heads, 32K keys, where two waves even out the heads, 290 and 275)
-  static constexpr int CTA_B = SMEM + (int)sizeof(Nodes) + 64 + 1024;
-  static constexpr int PER_SM = MINB * CTA_B <= 228 * 1024 ? MINB : 228 * 1024 / CTA_B;
-  static_assert(PER_SM >= 1 && PER_SM * CTA_B <= 228 * 1024, "a grid of PER_SM CTAs an SM is resident at once");
+  // CTAs resident on an SM (int8 rows of 128 with 17 to 32 nodes: one; 32 nodes, 4 x 8
+  // heads, 8K keys 47 us, 56 with runs cut for two; 24 nodes, 4 x 16 heads, 32K keys,
+  // where two waves even out the heads, 290 and 275)
+  static constexpr int PER_SM = fit_shared(SMEM, MINB);
+  static_assert(PER_SM >= 1 && sizeof(Nodes) + 64 <= 1536, "a CTA fits, and its static arrays are counted");
 };
 
 // Byte offset of 16-byte chunk c of row r in a tile: the XOR makes the fragment
