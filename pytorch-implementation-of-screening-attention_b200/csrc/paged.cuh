@@ -10,17 +10,20 @@ void commit(const screen_commit_args& a, cudaStream_t s);
 
 // Positions are cut into tiles of kTreeTile keys.
 constexpr int kTreeTile = 64;
-// Segments (sequence, head) of a call whose tiles are shared out over CTAs.
-constexpr int kTreeMaxShared = 2048;
+// CTAs of a shared-out call, at most: four on each of 148 SMs.  Its segments
+// (sequence, head) are fewer, or there is nobody to share with.
+constexpr int kTreeMaxCtas = 148 * 4;
 struct TreeParams {
   screen_tree_args a;
   int lens_off;   // added to a.lens (decode: -1, the query is the newest cached token)
   int part_off;   // floats of the workspace before the partial sums
 };
-void tree_bf16(const TreeParams& p, float* part, cudaStream_t s);
-void tree_i8(const TreeParams& p, float* part, cudaStream_t s);
-void tree_i8_f32(const TreeParams& p, float* part, cudaStream_t s);
-void tree_f32(const TreeParams& p, float* part, cudaStream_t s);
+// Each returns whether it shared the tiles out (num_ctas > 1 and more CTAs resident
+// than segments): tree_finish has to follow.
+bool tree_bf16(TreeParams p, float* part, cudaStream_t s);
+bool tree_i8(TreeParams p, float* part, cudaStream_t s);
+bool tree_i8_f32(TreeParams p, float* part, cudaStream_t s);
+bool tree_f32(TreeParams p, float* part, cudaStream_t s);
 void tree_finish(const TreeParams& p, const float* part, cudaStream_t s);
 
 void verify(const screen_verify_args& a, cudaStream_t s);

@@ -45,13 +45,6 @@ int tree_run(const screen_tree_args* a, int lens_off, cudaStream_t s) {
   if (!a->q || !a->lens || !a->r || !a->w || !a->y || (!a->k) != (!a->v))
     return SCREEN_ERR_INVALID_ARG;
   if ((long long)a->B * a->H > (1 << 28)) return SCREEN_ERR_UNSUPPORTED;
-  // more segments than the sharing out takes, or than CTAs: one CTA each
-  screen_tree_args one;
-  if (a->num_ctas > 1 && ((long long)a->B * a->H > kTreeMaxShared || (long long)a->B * a->H > a->num_ctas)) {
-    one = *a;
-    one.num_ctas = 1;
-    a = &one;
-  }
   int st = cache_ok(a->cache, a->cache_dtype, a->k_scales, a->v_scales);
   if (st) return st;
   if (!raw_ok(a->q, a->q_sb, a->q_st) || !al16(a->y)) return SCREEN_ERR_ALIGNMENT;
@@ -61,17 +54,16 @@ int tree_run(const screen_tree_args* a, int lens_off, cudaStream_t s) {
   if (need && (!a->workspace || a->workspace_bytes < need)) return SCREEN_ERR_WORKSPACE;
   if (need && !al16(a->workspace)) return SCREEN_ERR_ALIGNMENT;
   TreeParams p{*a, lens_off, (int)part_off(a)};
+  if (!need) p.a.num_ctas = 1;   // nobody to share with
+  bool shared;
   float* part = reinterpret_cast<float*>(a->workspace);
   if (a->cache_dtype == SCREEN_I8) {
-    if (a->dtype == SCREEN_F32) tree_i8_f32(p, part, s);
-    else tree_i8(p, part, s);
-  } else if (a->dtype == SCREEN_F32) {
-    tree_f32(p, part, s);
+    shared = a->dtype == SCREEN_F32 ? tree_i8_f32(p, part, s) : tree_i8(p, part, s);
   } else {
-    tree_bf16(p, part, s);
+    shared = a->dtype == SCREEN_F32 ? tree_f32(p, part, s) : tree_bf16(p, part, s);
   }
   st = check_launch();
-  if (st || a->num_ctas == 1) return st;
+  if (st || !shared) return st;
   tree_finish(p, part, s);
   return check_launch();
 }
@@ -114,7 +106,10 @@ int screen_paged_read(const screen_paged_read_args* a, screen_stream_t stream) {
 }
 
 size_t screen_tree_workspace_size(const screen_tree_args* a) {
-  if (!a || tree_checks(a) || a->num_ctas == 1) return 0;
+  if (!a || tree_checks(a)) return 0;
+  // as many segments as CTAs: one each, and no sums to join
+  const long long segs = (long long)a->B * a->H;
+  if (segs >= a->num_ctas || segs >= kTreeMaxCtas) return 0;
   return round_up((part_off(a) + (size_t)a->num_ctas * a->n * a->D) * sizeof(float));
 }
 

@@ -21,7 +21,9 @@
 // that are resident at once; it then takes its own run.  No host knowledge of
 // lengths or windows is needed.  A run that is not a whole segment leaves its sum
 // in the workspace slot of its CTA, and tree_finish_kernel adds a segment's slots
-// in order.  (Cutting the list of all tiles into equal runs instead gave some
+// in order.  Calls with as many segments as resident CTAs (444 or 592 for most forms,
+// 28 or 37 sequences of 16 heads) get a CTA per segment and are not cut: there the
+// longest segment sets the time.  (Cutting the list of all tiles into equal runs instead gave some
 // CTAs parts of two segments, and a part costs 6 us before its first tile.)  With
 // few tiles a segment goes to one CTA and no second launch follows.
 #pragma once
@@ -71,9 +73,8 @@ struct SegSlots {
   int first, count;
 };
 constexpr int kMinTiles = 4;         // a run is at least this long
-constexpr int kMaxShared = kTreeMaxShared;
 // This CTA's run: tiles [c0, c1] of segment seg.  False if there is none for it.
-// All threads of the CTA; `tiles` is kMaxShared ints of shared memory.
+// All threads of the CTA; `tiles` is kTreeMaxCtas ints of shared memory.
 __device__ __forceinline__ bool find_run(const TreeParams& p, int* tiles, SegSlots* slots, int& seg,
                                          Range& g, int& c0, int& c1, bool& whole) {
   const int segs = p.a.B * p.a.H, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -361,13 +362,14 @@ constexpr int fit_shared(size_t smem, int most) {
   return n < (size_t)most ? (int)n : most;
 }
 
-// One CTA per segment, or at most as many as are resident at once (a CTA per segment
-// at least).
-constexpr int kSMs = 148;
-inline dim3 tree_grid(const TreeParams& p, int per_sm) {
-  if (p.a.num_ctas == 1) return dim3(p.a.B * p.a.H);
-  const int segs = p.a.B * p.a.H, fit = kSMs * per_sm > segs ? kSMs * per_sm : segs;
-  return dim3(p.a.num_ctas < fit ? p.a.num_ctas : fit);
+// The grid: as many CTAs as are resident at once, num_ctas at most; one per segment,
+// and num_ctas = 1, if that is no more than the segments.
+inline dim3 tree_grid(TreeParams& p, int per_sm) {
+  const int segs = p.a.B * p.a.H, fit = kTreeMaxCtas / 4 * per_sm;
+  const int ctas = p.a.num_ctas < fit ? p.a.num_ctas : fit;
+  if (ctas > segs) return dim3(ctas);
+  p.a.num_ctas = 1;
+  return dim3(segs);
 }
 
 }  // namespace tree

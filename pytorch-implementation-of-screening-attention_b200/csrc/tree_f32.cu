@@ -166,15 +166,17 @@ __global__ void __launch_bounds__(128) tree_finish_kernel(TreeParams p, const fl
 }
 
 template <int D>
-void launch_f32(const TreeParams& p, float* part, cudaStream_t s) {
-  size_t smem = ((size_t)p.a.n * D + 2 * kKeys * (D + 4) + (size_t)p.a.n * 33) * 4;
-  if (smem < kMaxShared * 4) smem = kMaxShared * 4;   // find_run
+bool launch_f32(TreeParams& p, float* part, cudaStream_t s) {
+  const size_t smem = ((size_t)p.a.n * D + 2 * kKeys * (D + 4) + (size_t)p.a.n * 33) * 4;
+  static_assert(2 * kKeys * (D + 4) >= kTreeMaxCtas, "find_run works in it");
   constexpr int kMost = (kMaxN * D + 2 * kKeys * (D + 4) + kMaxN * 33) * 4;
-  if (ensure_smem_optin((const void*)tree_f32_kernel<D>, kMost) != cudaSuccess) return;
+  if (ensure_smem_optin((const void*)tree_f32_kernel<D>, kMost) != cudaSuccess) return false;
   prefer_shared((const void*)tree_f32_kernel<D>);
   // three CTAs an SM where they fit (64 nodes of 128: two)
   static_assert(sizeof(Nodes) + kKeys * 12 + 64 <= 1536, "the static arrays are counted");
-  launch_pdl(tree_f32_kernel<D>, tree_grid(p, fit_shared(smem, 3)), dim3(kThreads), smem, s, p, part);
+  const dim3 grid = tree_grid(p, fit_shared(smem, 3));
+  launch_pdl(tree_f32_kernel<D>, grid, dim3(kThreads), smem, s, p, part);
+  return p.a.num_ctas > 1;
 }
 template <typename TA, int D>
 void launch_finish(const TreeParams& p, const float* part, cudaStream_t s) {
@@ -195,12 +197,12 @@ void finish_d(const TreeParams& p, const float* part, cudaStream_t s) {
 }  // namespace
 }  // namespace tree
 
-void tree_f32(const TreeParams& p, float* part, cudaStream_t s) {
+bool tree_f32(TreeParams p, float* part, cudaStream_t s) {
   switch (p.a.D) {
-    case 16: tree::launch_f32<16>(p, part, s); break;
-    case 32: tree::launch_f32<32>(p, part, s); break;
-    case 64: tree::launch_f32<64>(p, part, s); break;
-    case 128: tree::launch_f32<128>(p, part, s); break;
+    case 16: return tree::launch_f32<16>(p, part, s);
+    case 32: return tree::launch_f32<32>(p, part, s);
+    case 64: return tree::launch_f32<64>(p, part, s);
+    default: return tree::launch_f32<128>(p, part, s);
   }
 }
 void tree_finish(const TreeParams& p, const float* part, cudaStream_t s) {

@@ -2,7 +2,7 @@
 // (tree_mma.cuh).
 #include "tree_mma.cuh"
 namespace screen {
-void tree_i8(const TreeParams& p, float* part, cudaStream_t s) {
-  tree::launch_tree_e<signed char, __nv_bfloat16>(p, part, s);
+bool tree_i8(TreeParams p, float* part, cudaStream_t s) {
+  return tree::launch_tree_e<signed char, __nv_bfloat16>(p, part, s);
 }
 }  // namespace screen

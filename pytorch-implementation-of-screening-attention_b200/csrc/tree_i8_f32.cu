@@ -2,7 +2,7 @@
 // (tree_mma.cuh): the query and alpha enter the products as hi + lo halves.
 #include "tree_mma.cuh"
 namespace screen {
-void tree_i8_f32(const TreeParams& p, float* part, cudaStream_t s) {
-  tree::launch_tree_e<signed char, float>(p, part, s);
+bool tree_i8_f32(TreeParams p, float* part, cudaStream_t s) {
+  return tree::launch_tree_e<signed char, float>(p, part, s);
 }
 }  // namespace screen

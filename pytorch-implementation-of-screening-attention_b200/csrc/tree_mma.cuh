@@ -100,8 +100,8 @@ struct Cfg {
   static constexpr int GROUP_B = (PLAN_AT + PLAN_B + 15) / 16 * 16;
   static constexpr int RED_B = 4 * 16 * D_ * 4;       // the warps' sums at the end
   static constexpr int MAIN_B = WK * GROUP_B > RED_B ? WK * GROUP_B : RED_B;
-  static constexpr int SMEM = MAIN_B > kMaxShared * 4 ? MAIN_B : kMaxShared * 4;
-  static_assert(SMEM >= kAppendScratch && SMEM >= kMaxShared * 4, "append_rows and find_run work in it");
+  static constexpr int SMEM = MAIN_B > kAppendScratch ? MAIN_B : kAppendScratch;
+  static_assert(SMEM >= kAppendScratch && SMEM >= kTreeMaxCtas * 4, "append_rows and find_run work in it");
   // CTAs per SM the registers are cut to: what a thread holds of O and q decides
   static constexpr int HELD = D_ / 2 + D_ / 4 * (QHL ? 2 : 1);
   // (a group of four warps on int8 pages waits at its barriers and gains by a fourth
@@ -919,27 +919,29 @@ __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams 
 }
 
 template <class C>
-void launch_tree(const TreeParams& p, float* ws, cudaStream_t s) {
-  if (ensure_smem_optin((const void*)tree_mma_kernel<C>, C::SMEM) != cudaSuccess) return;
+bool launch_tree(TreeParams& p, float* ws, cudaStream_t s) {
+  if (ensure_smem_optin((const void*)tree_mma_kernel<C>, C::SMEM) != cudaSuccess) return false;
   prefer_shared((const void*)tree_mma_kernel<C>);
-  launch_pdl(tree_mma_kernel<C>, tree_grid(p, C::PER_SM), dim3(kThreads), (size_t)C::SMEM, s, p, ws);
+  const dim3 grid = tree_grid(p, C::PER_SM);
+  launch_pdl(tree_mma_kernel<C>, grid, dim3(kThreads), (size_t)C::SMEM, s, p, ws);
+  return p.a.num_ctas > 1;
 }
 // A warp for every 16 queries; up to 8 queries the lower half of a tile is not
 // computed on.
 template <typename E, typename TA, int D>
-void launch_tree_d(const TreeParams& p, float* ws, cudaStream_t s) {
-  if (p.a.n <= 8) launch_tree<Cfg<E, TA, D, 1, 1>>(p, ws, s);
-  else if (p.a.n <= 16) launch_tree<Cfg<E, TA, D, 1, 2>>(p, ws, s);
-  else if (p.a.n <= 32) launch_tree<Cfg<E, TA, D, 2, 2>>(p, ws, s);
-  else launch_tree<Cfg<E, TA, D, 4, 2>>(p, ws, s);
+bool launch_tree_d(TreeParams& p, float* ws, cudaStream_t s) {
+  if (p.a.n <= 8) return launch_tree<Cfg<E, TA, D, 1, 1>>(p, ws, s);
+  if (p.a.n <= 16) return launch_tree<Cfg<E, TA, D, 1, 2>>(p, ws, s);
+  if (p.a.n <= 32) return launch_tree<Cfg<E, TA, D, 2, 2>>(p, ws, s);
+  return launch_tree<Cfg<E, TA, D, 4, 2>>(p, ws, s);
 }
 template <typename E, typename TA>
-void launch_tree_e(const TreeParams& p, float* ws, cudaStream_t s) {
+bool launch_tree_e(TreeParams& p, float* ws, cudaStream_t s) {
   switch (p.a.D) {
-    case 16: launch_tree_d<E, TA, 16>(p, ws, s); break;
-    case 32: launch_tree_d<E, TA, 32>(p, ws, s); break;
-    case 64: launch_tree_d<E, TA, 64>(p, ws, s); break;
-    case 128: launch_tree_d<E, TA, 128>(p, ws, s); break;
+    case 16: return launch_tree_d<E, TA, 16>(p, ws, s);
+    case 32: return launch_tree_d<E, TA, 32>(p, ws, s);
+    case 64: return launch_tree_d<E, TA, 64>(p, ws, s);
+    default: return launch_tree_d<E, TA, 128>(p, ws, s);
   }
 }
 

@@ -228,13 +228,17 @@ def paged_read(positions, n: int, k_pages, v_pages, block_table, k_scales=None, 
     return k, v
 
 
+_MAX_CTAS = 148 * 4          # of a tree call that are resident at once, at most
+
+
 def _tree_ctas(bh: int, keys: int) -> int:
     """CTAs that the 64-key tiles of a call are shared out over, at most (the
     library takes as many as run at once); 1: one for each of the bh (sequence,
-    head) pairs, and no second launch."""
-    if keys // 64 + 2 <= 8 or bh > 2048:
+    head) pairs, and no second launch.  From as many pairs as resident CTAs on the
+    library takes one each in any case."""
+    if keys // 64 + 2 <= 8 or bh >= _MAX_CTAS:
         return 1
-    return 148 * 4
+    return _MAX_CTAS
 
 
 def _keys_seen(max_window, block_table, page_size):
@@ -308,8 +312,8 @@ def _tree(name, q, k, v, lens, parents, r, w, k_pages, v_pages, block_table, k_s
             y.data_ptr())
     if num_ctas > 1:
         need = _size_query("screen_tree_workspace_size")(pack(*args, 0, 0))
-        ws = torch.UntypedStorage(need, device=q.device)
-        _run(call, pack(*args, ws.data_ptr(), need), index)
+        ws = torch.UntypedStorage(need, device=q.device) if need else None
+        _run(call, pack(*args, ws.data_ptr() if need else 0, need), index)
     else:
         _run(call, pack(*args, 0, 0), index)
     return y

@@ -502,3 +502,35 @@ def test_decode_queries_that_start_anywhere(ms, dtype):
     want = ms.paged_decode(q, *tail)
     assert torch.equal(ms.paged_decode(flat[1:].view(1, 3, 64), *tail), want)
     assert torch.equal(ms.paged_decode(q.as_strided((1, 3, 64), (7, 64, 1)), *tail), want)
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)])
+@pytest.mark.parametrize("B,H", [(31, 16), (41, 17), (70, 30)])
+def test_more_pairs_than_resident_ctas(ms, B, H, dtype, q8):
+    """Around and beyond one (sequence, head) pair per resident CTA, uneven lengths:
+    any num_ctas gives each pair to one CTA, the bits of num_ctas = 1, which are
+    those of its sequence alone."""
+    D, ps, T, n = 16, 16, 300, 3
+    c = make(ms, B, H, D, ps, T, n, dtype, q8, B)
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, T, (B,), generator=g).to(torch.int32)
+    lens[3] = T
+    lens[5] = -1
+    r, w = torch.full((H,), 1.1), torch.linspace(T + 5.0, 9.0, H)
+    dev = [x.to(DEV) for x in (c["q"], c["k"], c["v"], lens)]
+    rw = (r.to(DEV), w.to(DEV))
+
+    def run(lo=0, hi=B, **kw):
+        part = [x[lo:hi] for x in dev]
+        return ms.paged_tree_decode(*part, None, *rw, c["kp"], c["vp"], c["table"][lo:hi], c["ks"], c["vs"], **kw)
+
+    want = run(num_ctas=1)
+    assert (want[5] == 0).all() and want.isfinite().all()
+    for kw in (dict(), dict(num_ctas=B * H), dict(num_ctas=60000)):
+        got = run(**kw)
+        if B * H >= 592 or kw.get("num_ctas") == B * H:
+            assert torch.equal(got, want), kw
+        else:                                    # 496 pairs: four CTAs an SM share out, three do not
+            tol = 2.0**-6 if dtype == torch.bfloat16 else 2.0**-17
+            assert ((got - want).float().norm(dim=-1) <= tol * want.float().norm(dim=-1) + 1e-6).all()
+    assert torch.equal(run(2, 6, num_ctas=1), want[2:6])
