@@ -12,6 +12,7 @@ prefix for every token (multiscreen/model.py:131-133).
 """
 from __future__ import annotations
 
+import ctypes
 import math
 import struct
 
@@ -23,30 +24,36 @@ _PAGE_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.int8: 
 MAX_NODES = _lib.TREE_MAX_NODES
 
 # A call's arguments are packed straight into the bytes of its C struct
-# (include/screening_b200.h; native alignment): building the ctypes mirror field by
-# field cost as much as the shortest of these kernels runs.  _entry() checks the
-# sizes against the mirrors.
-_CACHE = "3P4i"
-_LAYOUTS = {
-    "screen_kv_append": ("5if P2q P2q P" + _CACHE + "0q", _lib.KVAppendArgs),
-    "screen_paged_append_i8": ("5if P2q P2q P" + _CACHE + "2P0q", _lib.PagedAppendArgs),
-    "screen_paged_read": ("6i2P P" + _CACHE + "2P0q", _lib.PagedReadArgs),
-    "screen_tree_decode": ("7if P2q P2q P2q 2Pq 2P" + _CACHE + "2P 2PN0q", _lib.TreeArgs),
-    "screen_paged_commit": ("6i 2PqP" + _CACHE + "2Pq0q", _lib.CommitArgs),
-    "screen_verify_drafts": ("4ifi P P2q P2q Pq Pq Pq 3P PN0q", _lib.VerifyArgs),
+# (include/screening_b200.h; native alignment) in the order of the struct's ctypes
+# mirror: building the mirror field by field cost as much as the shortest of these
+# kernels runs.
+_STRUCTS = {
+    "screen_kv_append": _lib.KVAppendArgs,
+    "screen_paged_append_i8": _lib.PagedAppendArgs,
+    "screen_paged_read": _lib.PagedReadArgs,
+    "screen_tree_decode": _lib.TreeArgs,
+    "screen_paged_decode_i8": _lib.TreeArgs,
+    "screen_paged_commit": _lib.CommitArgs,
+    "screen_verify_drafts": _lib.VerifyArgs,
 }
-_LAYOUTS["screen_paged_decode_i8"] = _LAYOUTS["screen_tree_decode"]
+_CODES = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_void_p: "P",
+          ctypes.c_size_t: "N"}
 _entries = {}
+
+
+def _layout(mirror) -> str:
+    """The fields of a ctypes struct as struct codes, those of nested structs in line."""
+    return "".join(_layout(t) if issubclass(t, ctypes.Structure) else _CODES[t]
+                   for _, t in mirror._fields_)
 
 
 def _entry(name):
     """(pack, call) of a C entry point."""
     e = _entries.get(name)
     if e is None:
-        import ctypes
         lib = _lib.load()
-        fmt, mirror = _LAYOUTS[name]
-        st = struct.Struct(fmt.replace(" ", ""))
+        mirror = _STRUCTS[name]
+        st = struct.Struct(_layout(mirror) + "0q")
         if st.size != ctypes.sizeof(mirror):
             raise RuntimeError(f"{name}: packed arguments differ from {mirror.__name__}")
         proto = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)
@@ -58,7 +65,6 @@ def _size_query(name):
     """A workspace size query on packed arguments."""
     q = _entries.get(name)
     if q is None:
-        import ctypes
         proto = ctypes.CFUNCTYPE(ctypes.c_size_t, ctypes.c_char_p)
         q = _entries[name] = proto(ctypes.cast(getattr(_lib.load(), name), ctypes.c_void_p).value)
     return q
