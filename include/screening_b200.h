@@ -351,7 +351,9 @@ typedef struct screen_verify_args {
   int32_t B, n, V;               /* 0 <= n <= SCREEN_TREE_MAX_NODES           */
   float temperature;             /* > 0; 0: greedy (the first maximum)        */
   int32_t _pad0;
-  const float* temperatures;     /* (B,), or NULL: `temperature` for all      */
+  const float* temperatures;     /* (B,), or NULL: `temperature` for all;     */
+                                 /*   < 0 or NaN: a sequence without a        */
+                                 /*   distribution                            */
   const void* logits; int64_t l_sb, l_st;        /* (B,n+1,V)                 */
   const void* draft_logits; int64_t d_sb, d_st;  /* (B,n,V) or NULL           */
   const int64_t* tokens; int64_t t_sb;           /* (B,n) drafted tokens      */

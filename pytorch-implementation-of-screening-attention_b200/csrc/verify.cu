@@ -306,8 +306,8 @@ __device__ RowSum row_part(const T* row, const Part& t, int V, double c2, const 
 __device__ __forceinline__ float temp_of(const screen_verify_args& a, int b) {
   return a.temperatures ? a.temperatures[b] : a.temperature;
 }
-// log2(e) / T; T not above 0 means the maximum only (any positive T then tells
-// whether the row is usable).  T counts as 1e30 above that: -inf, held as -2^128,
+// log2(e) / T; T = 0 means the maximum only (any positive T then tells whether the row
+// is usable), below 0 or NaN nothing.  T counts as 1e30 above that: -inf, held as -2^128,
 // keeps the weight 0.
 __device__ __forceinline__ double scale_of(float temp) {
   return 1.4426950408889634 / (temp > 0.f ? fmin((double)temp, 1e30) : 1.0);
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(kT, 2) walk_kernel(screen_verify_args a, const
     RowSum P, Q;
     double before, mine;                          // parts of the last residual's sum
     w.rows(cur, prow, qrow, P, Q, before, mine);
-    if (!usable(P)) break;                        // no distribution: no token
+    if (!usable(P) || !(temp >= 0.f)) break;      // no distribution: no token
     if (qrow && !usable(Q)) left = 0;             // nothing was drawn from this
     const double mp = wide(P.m), mq = wide(Q.m);
     double c = 0.0, z = 1.0, all = P.s, out_mass = 0.0;

@@ -436,8 +436,10 @@ def verify_drafts(logits, tokens, parents, uniforms, draft_logits=None, temperat
     drafted token i.  tokens (B, n) int64, parents (B, n) int32 as in
     paged_tree_decode (None: a chain), uniforms (B, n + 1) float32 in [0, 1).
     draft_logits (B, n, V): row j is the distribution the children of row j were
-    drawn from; None: the tokens were picked, not drawn.  temperature: a float,
-    or a float32 (B,) tensor; 0 is greedy (the first maximum), above 1e30 counts as 1e30.
+    drawn from; None: the tokens were picked, not drawn.  temperature: a finite
+    float that is not negative, or a float32 (B,) tensor; 0 is greedy (the first
+    maximum), above 1e30 counts as 1e30.  A sequence whose entry is negative or NaN
+    has no distribution.
 
     Nodes are scanned in order, starting at row 0 with c = 0 and Z = 1.  A node
     whose parent is the current row is accepted iff u q(x) Z < p(x) - c q(x), p

@@ -203,3 +203,29 @@ def test_temperatures_near_zero_and_huge(ms, B, V, drawn, dtype):
 def test_tiny_temperatures_per_sequence(ms, tiny):
     c = case(3, 2, 301, "chain", True, 1.0, torch.float32, 9)
     check(ms, c, torch.tensor([tiny, 1.0, 0.0]).to(DEV))
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("B,V", [(6, 501), (60, 50257)])
+def test_temperatures_that_are_none(ms, B, V, drawn):
+    """A negative or NaN temperature, refused as a float, gives its sequence no token
+    as a tensor's entry; the others are as they were, an infinite one as 1e30."""
+    c = case(B, 3, V, "chain", drawn, 1.0, torch.float32, 21)
+    c["uniforms"][:, :3] = 0.0
+    temps = torch.ones(B)
+    temps[5] = 1e30
+    dev = {k: None if x is None else x.to(DEV) for k, x in c.items()}
+
+    def run(t):
+        return ms.verify_drafts(dev["logits"], dev["tokens"], None, dev["uniforms"], draft_logits=dev["draft_logits"],
+                                temperature=t.to(DEV))
+
+    want = run(temps)
+    bad = torch.tensor([1, 3, 4])
+    temps[1], temps[3], temps[4], temps[5] = -0.5, math.nan, -math.inf, math.inf
+    out, path, counts = run(temps)
+    keep = torch.ones(B, dtype=torch.bool)
+    keep[bad] = False
+    for x, y in zip((out, path, counts), want):
+        assert torch.equal(x[keep], y[keep])
+    assert (out[bad] == -1).all() and (path[bad] == -1).all() and (counts[bad] == 0).all()
