@@ -200,8 +200,10 @@ class MultiscreenLM(nn.Module):
         values are left in the cache at lens[b] + i.  parents as in
         paged_tree_decode, None for a chain; depths (B,n): the nodes' depths if
         they are at hand.  Node i of a chain sees what decode_step would at
-        position lens[b] + i.  After verify_drafts, cache.commit keeps the
-        accepted path (a chain's is in place)."""
+        position lens[b] + i; a node past max_seq_len takes the last position
+        embedding, and a negative token (an absent node's) is looked up as 0: what
+        such nodes yield is to be dropped.  After verify_drafts, cache.commit keeps
+        the accepted path (a chain's is in place)."""
         B, n = tokens.shape
         if state is None:
             state = self._decode_state()

@@ -190,7 +190,8 @@ def paged_append(k, v, positions, k_pages, v_pages, block_table, k_scales=None, 
     (int32).  int8 pages hold m = round_half_even(127 x / max|x|) and the scale
     1 / max(|m|, 127 eps / max|x|) per row, so that scale * m is a unit row; k, v
     are then float32 or bfloat16, otherwise of the pages' dtype.  Positions
-    outside the block table are skipped."""
+    outside the block table are skipped.  The rows of one call have to lie on
+    different rows of the pages: of a ring table, n is at most the ring's rows."""
     index, code, shape, cache, scales = _pages(k_pages, v_pages, block_table, k_scales, v_scales)
     if k.dim() != 4 or v.dtype is not k.dtype:
         raise ValueError("k and v must be (B, n, H, D) of one dtype")

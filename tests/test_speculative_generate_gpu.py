@@ -270,3 +270,20 @@ def test_int32_prompts(ms, graph):
     want = m.generate(ids.int(), 9, top_k=1)
     got = m.generate_speculative(ids.int(), d, 9, num_draft=3, temperature=0.0, cuda_graph=graph)
     assert got.dtype == want.dtype and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tree_step_near_the_end(ms, dtype):
+    """Nodes past max_seq_len and absent nodes with negative tokens leave the others'
+    logits alone."""
+    m = lm(ms, dtype, max_len=24)
+    ids = torch.randint(0, 97, (2, 22), device=DEV, generator=torch.Generator(device=DEV).manual_seed(8))
+    lens = torch.full((2,), 22, dtype=torch.int32, device=DEV)
+    tokens = torch.tensor([[5, 6, 7, -1], [8, 9, 10, -1]], device=DEV)
+    parents = torch.tensor([[-1, 0, 1, -2]] * 2, dtype=torch.int32, device=DEV)
+    caches = [m.make_cache(2, 30, max_draft=3) for _ in range(2)]
+    for c in caches:
+        m.prefill(ids, c)
+    a = m.tree_step(tokens, lens, caches[0], parents=parents)
+    b = torch.stack([m.decode_step(tokens[:, i:i + 1], lens + i, caches[1]) for i in range(2)], 1)
+    assert a.isfinite().all() and rel_err(a[:, :2].float(), b.float()) <= TOL[dtype]
