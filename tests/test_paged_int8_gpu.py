@@ -229,3 +229,22 @@ def test_more_heads_than_a_block_moves_at_once(ms, dtype, H):
         want = m.double() * sc[..., None]
         assert ((val.double().cpu() - want).abs() <= 4 * 2.0**-24 * want.abs()).all()
     assert int((kp != 7).any(-1).sum()) <= B * n * H
+
+
+@pytest.mark.parametrize("page,out", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                      (torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("H,D,ps", [(3, 16, 8), (5, 128, 24), (70, 64, 16)])
+def test_read_of_other_pages(ms, H, D, ps, page, out):
+    B, n = 2, 37
+    g = torch.Generator().manual_seed(H)
+    P = B * 4
+    table = torch.randperm(P, generator=g).view(B, 4).to(torch.int32)
+    table[1, 2] = -1
+    kp, vp = (torch.randn(P, H, ps, D, generator=g).to(page) for _ in range(2))
+    pos = torch.tensor([-3, ps - 1], dtype=torch.int32)
+    got = ms.paged_read(pos.to(DEV), n, kp.to(DEV), vp.to(DEV), table.to(DEV), dtype=out)
+    for pages, x in zip((kp, vp), got):
+        assert x.dtype == out and x.shape == (B, n, H, D)
+        for b in range(B):
+            want = po.cache_values(pages, None, table, b, [int(pos[b]) + i for i in range(n)]).nan_to_num(0.0)
+            assert torch.equal(x[b].cpu(), want.float().to(out))

@@ -534,3 +534,59 @@ def test_more_pairs_than_resident_ctas(ms, B, H, dtype, q8):
             tol = 2.0**-6 if dtype == torch.bfloat16 else 2.0**-17
             assert ((got - want).float().norm(dim=-1) <= tol * want.float().norm(dim=-1) + 1e-6).all()
     assert torch.equal(run(2, 6, num_ctas=1), want[2:6])
+
+
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False),
+                                      (torch.float32, True)])
+@pytest.mark.parametrize("n,ctas", [(1, 1), (7, 40), (20, 1), (40, 592)])
+def test_rows_that_are_there_already(ms, n, ctas, dtype, q8):
+    """k, v = None: the nodes' rows were appended before.  The same bits, and nothing is
+    written."""
+    c = make(ms, 2, 2, 64, 24, 150, n, dtype, q8, 60 + n)
+    lens = torch.tensor([150, 90], dtype=torch.int32, device=DEV)
+    parents = tree_parents(2, n, "random", c["g"]).to(DEV)
+    r, w = torch.tensor([1.1, 1.4], device=DEV), torch.tensor([120.0, 33.0], device=DEV)
+    q, k, v = (c[x].to(DEV) for x in "qkv")
+    rest = (lens, parents, r, w, c["kp"], c["vp"], c["table"], c["ks"], c["vs"])
+    want = ms.paged_tree_decode(q, k, v, *rest, num_ctas=1)
+    held = [None if c[x] is None else c[x].clone() for x in ("kp", "vp", "ks", "vs")]
+    ms.paged_append(k, v, lens, c["kp"], c["vp"], c["table"], c["ks"], c["vs"])
+    assert all(x is None or torch.equal(x, c[y]) for x, y in zip(held, ("kp", "vp", "ks", "vs")))
+    got = ms.paged_tree_decode(q, None, None, *rest, num_ctas=ctas)
+    if ctas == 1:
+        assert torch.equal(got, want)
+    else:
+        tol = 2.0**-7 if dtype == torch.bfloat16 else 2.0**-18
+        assert ((got - want).float().norm(dim=-1) <= tol * want.float().norm(dim=-1) + 1e-6).all()
+    assert all(x is None or torch.equal(x, c[y]) for x, y in zip(held, ("kp", "vp", "ks", "vs")))
+
+
+@pytest.mark.parametrize("eps", [1e-8, 0.5, 30.0])
+@pytest.mark.parametrize("dtype,q8", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False),
+                                      (torch.float32, True)])
+def test_rows_and_queries_below_eps(ms, dtype, q8, eps):
+    """Raw rows of norm about 8 and 0: eps holds short rows, queries and sums down."""
+    B, H, D, ps, T, n = 2, 2, 64, 16, 40, 5
+    c = make(ms, B, H, D, ps, T, n, dtype, q8, 5)
+    c["q"][0, 1] = 0
+    c["k"][0, 2] = 0
+    c["v"][1, 0] = 0
+    lens = torch.tensor([T, 20], dtype=torch.int32)
+    r, w = torch.tensor([0.9, 0.6]), torch.tensor([30.0, 12.0])
+    dev = [c[x].to(DEV) for x in "qkv"] + [lens.to(DEV), None, r.to(DEV), w.to(DEV)]
+    prefix = tuple(None if x is None else x.cpu().clone() for x in (c["kp"], c["vp"], c["ks"], c["vs"], c["table"]))
+    y = ms.paged_tree_decode(*dev, c["kp"], c["vp"], c["table"], c["ks"], c["vs"], eps=eps)
+    for b in range(B):
+        held = []
+        for x in "kv":
+            got = po.cache_values(c[x + "p"], c[x + "s"], c["table"], b, [int(lens[b]) + i for i in range(n)])
+            if q8:
+                m, sc = po.int8_rows(c[x][b], eps)
+                row, tol = m.double() * sc[..., None], 2.0**-21
+            else:
+                row, tol = po.unit_rows(c[x][b], eps), 2.0**-21 + (2.0**-8 if dtype == torch.bfloat16 else 0.0)
+            assert ((got - row).abs() <= tol * row.abs() + 1e-12).all()
+            held.append(got)
+        want, sums = po.tree(c["q"][b], held[0], held[1], int(lens[b]), None, r, w, prefix, b, eps)
+        err = (y[b].double().cpu() - want).norm(dim=-1)
+        assert (err <= bound(want, sums, r, dtype, q8)).all(), (b, err)
