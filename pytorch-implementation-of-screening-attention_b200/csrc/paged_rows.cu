@@ -202,8 +202,9 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(screen_paged_read_
 // per (layer, K / V, sequence, head).  All source rows are staged in shared
 // memory before the first write, so any path is right, and rows that stay
 // where they are (a chain's) are not touched.  Bound by latency: lengths, path, table
-// and rows one after another, 3.6 us for 12 layers of a tree of 16 on bf16 pages, 8.2
-// us for 64 rows on int8 pages (2 us of traffic).
+// and rows one after another, 3.6 us for 12 layers of a tree of 16 on bf16 pages, 8.1
+// us for 64 rows of 8 x 16 heads on int8 pages (2 us of traffic; 3072 CTAs, 1.7 times
+// those resident at once).
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(128) commit_kernel(screen_commit_args a, int row_bytes) {
   pdl_wait();

@@ -92,7 +92,7 @@ __device__ __forceinline__ bool find_run(const TreeParams& p, int* tiles, SegSlo
   const int ctas = gridDim.x;
   long long sum = 0;
   // writing the nodes' rows takes the time of about a tile per 16 of them, behind a
-  // segment's last (counted so, 64 nodes over 32K keys: 136 us, not counted 142)
+  // segment's last (counted so, 64 nodes over 32K keys: 157 us, not counted 164)
   const int extra = p.a.k ? (p.a.n + 15) / 16 : 0;
   for (int j = tid; j < segs; j += kThreads) {
     const Range rg = tree_range(p, j / p.a.H, j % p.a.H);

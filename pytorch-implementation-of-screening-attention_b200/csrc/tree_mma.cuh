@@ -292,9 +292,11 @@ __device__ __forceinline__ void widen16(uint4 u, uint4& lo, uint4& hi) {
 //
 // A group of one warp (up to 16 nodes) is bound by its issue and its waits before
 // HBM: one query per sequence over 100K int8 keys of 64 heads 122 us, 4.5 TB/s.  64
-// nodes over 32K int8 keys 157 us, 137 TFLOP/s (135 us with alpha as one fp16 number,
-// whose rounding showed where values cancel).  16 nodes over
-// windows of 4K on bf16 pages 24 us, 8.2 us for one token over 256 int8 keys: latency.
+// nodes over 32K int8 keys 157 us, 137 TFLOP/s, half of the issue slots and 40 % of
+// mma.sync used (490 instructions a warp per 32 keys x 16 nodes; 136 us and 430 with
+// alpha as one fp16 number).  64 nodes over 32K bf16 keys 178 us (151 with alpha as
+// two bf16 numbers).  16 nodes over windows of 4K on bf16 pages 25 us, 8.1 us for one
+// token over 256 int8 keys: latency.
 template <class C>
 __global__ void __launch_bounds__(kThreads, C::MINB) tree_mma_kernel(TreeParams p,
                                                                      float* __restrict__ ws) {

@@ -24,7 +24,7 @@
 //
 // Bound by the passes of a walk, one after another, each a row through the 64-bit
 // units of a cluster's SMs: 4 chains of 4 with drafting logits over 50257 tokens 24
-// us, 32 trees of 32 34 us.
+// us, 32 trees of 32 34 us; greedy, where only the sums' health is used, 14 and 28 us.
 //
 // Sums are in 64 bits throughout: with 50K tokens of probability 1e-5 a running
 // sum in 32 bits would often cross u one token away, and an acceptance test next
