@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(screen_paged_read_
 // memory before the first write, so any path is right, and rows that stay
 // where they are (a chain's) are not touched.  Bound by latency: lengths, path, table
 // and rows one after another, 3.6 us for 12 layers of a tree of 16 on bf16 pages, 8.1
-// us for 64 rows of 8 x 16 heads on int8 pages (2 us of traffic; 3072 CTAs, 1.7 times
-// those resident at once).
+// us for 64 rows of 8 x 16 heads on int8 pages (2 us of traffic; 1.7 times as many
+// CTAs as are resident at once).
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(128) commit_kernel(screen_commit_args a, int row_bytes) {
   pdl_wait();
