@@ -300,6 +300,8 @@ typedef struct screen_tree_args {
   int32_t num_ctas;              /* 1: one CTA per (sequence, head); more:    */
                                  /*   all key tiles are shared out over that  */
                                  /*   many CTAs, a second pass adds the parts */
+                                 /*   (at most those resident at once; one    */
+                                 /*   each where no more than the pairs)      */
   float eps;
   const void* q; int64_t q_sb, q_st;   /* raw (B,n,H,D)                       */
   const void* k; int64_t k_sb, k_st;   /* raw rows of the nodes, or NULL:     */
@@ -314,6 +316,7 @@ typedef struct screen_tree_args {
   void* workspace; size_t workspace_bytes;
 } screen_tree_args;
 
+/* 0 where nothing is shared out. */
 SCREEN_API size_t screen_tree_workspace_size(const screen_tree_args* a);
 
 /* Screening attention of a tree of n drafted tokens per sequence.  Node i has
